@@ -1,7 +1,9 @@
 /*
  * nnop_b200.h -- C ABI of the B200 (sm_100a) implementation of NNop's fused
  * kernels: flash attention (forward/backward, pair bias, causal, GQA,
- * key-padding mask), online softmax, RMSNorm, LayerNorm and Llama RoPE.
+ * key-padding mask), online softmax, RMSNorm, LayerNorm and Llama RoPE; and
+ * of a paged key-value cache beside them (append, attention of one new token,
+ * eviction by accumulated attention weight).
  *
  * Conventions (all entry points)
  * ------------------------------
@@ -418,6 +420,111 @@ int nnop_llama_rope(const void* q, const void* k,
 int nnop_llama_rope_cos_sin(const float* position_ids, float* cos_t, float* sin_t,
                             int64_t dim, int64_t L, int64_t B, int64_t base,
                             void* stream);
+
+/* --------------------------------------------------------------------------
+ * Paged key-value cache.  No counterpart in the reference, whose attention
+ * (src/attention.jl:145-197) takes whole sequences; these serve the step after
+ * it, one new token against the keys and values kept so far.
+ *
+ * Arguments the three calls share:
+ *   k_cache, v_cache  [pages][KH][page_size][E] dtype (Julia (E, page_size, KH,
+ *                     pages)): the pools.  page_stride, head_stride, row_stride
+ *                     are the element strides of the first three dimensions,
+ *                     the same for both pools, multiples of 16 bytes (contiguous
+ *                     pools: KH*page_size*E, page_size*E, E); E is contiguous.
+ *   block_table       [B][max_pages] int32 (Julia (max_pages, B)): the page of
+ *                     each run of page_size slots of a sequence.  An entry
+ *                     outside [0, pages) is no page: its slots are not attended
+ *                     to, and rows meant for them are dropped.
+ *   lengths           [B] int32: slots in use, taken as within
+ *                     [0, max_pages*page_size].
+ * E is 16, 32, 64 or 128; dtype F32, F16 or BF16; q, k, v, o and the pools are
+ * 16-byte aligned; at most 2^31 - 1024 pages, and slots per sequence.  Page
+ * numbers and lengths are read on the device, so a captured graph replays with
+ * what they hold then.  A contiguous cache [B][KH][L][E] is a pool of pages of
+ * L slots with the table [[0], [1], ..., [B - 1]].
+ * -------------------------------------------------------------------------- */
+
+/*
+ * Appends new rows: row t < n_new[b] (n_new NULL: all T; taken as within
+ * [0, T]) of k and v goes to slot lengths[b] + t of sequence b.  Rows past the
+ * table's last slot are dropped.  Nothing else of the pools is written.
+ *   k, v [B][KH][T][E]; new_lengths [B] = min(lengths + n_new, slots), not
+ *   the array `lengths` itself.
+ *   cos_t, sin_t [cos_batch][T][E] f32 (cos_batch = 1 or B) or both NULL: k is
+ *   rotated on its way as nnop_llama_rope rotates it, bit for bit, and with
+ *   QH > 0 so are the queries q [B][QH][T][E] into q_out (all T of them).
+ *   Without cos/sin: QH = 0, q and q_out NULL.
+ * A page that rows go to belongs to one sequence and stands in its table once
+ * (else which of two rows remains is left open).
+ */
+int nnop_paged_append(const void* q, const void* k, const void* v,
+                      const float* cos_t, const float* sin_t,
+                      const int32_t* n_new, void* q_out,
+                      void* k_cache, void* v_cache,
+                      const int32_t* block_table, const int32_t* lengths,
+                      int32_t* new_lengths,
+                      int64_t E, int64_t T, int64_t QH, int64_t KH, int64_t B,
+                      int64_t cos_batch,
+                      int64_t pages, int64_t page_size, int64_t max_pages,
+                      int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                      int dtype, void* stream);
+
+/* Bytes of workspace nnop_paged_attention_fwd needs (has_weights: weights will
+ * be passed). */
+size_t nnop_paged_attention_fwd_workspace_size(int64_t E, int64_t QH, int64_t KH, int64_t B,
+                                               int64_t page_size, int64_t max_pages,
+                                               int has_weights, int dtype);
+
+/*
+ * Attention of one new token per sequence over the slots j < lengths[b] that
+ * have a page: nnop_flash_attention_fwd with QL = 1 and the sequence's cached
+ * rows as k and v (same scale, same query-head groups).
+ *   q, o [B][QH][E] (QL = 1: the flash-attention layout [B][QH][1][E]);
+ *   lse [B][QH] f32.  A sequence without a slot (or whose scores are all -Inf)
+ *   gets o = 0, lse = -Inf.
+ *   weights [B][KH][max_pages*page_size] f32 or NULL: for every attended slot j
+ *   weights[b][h][j] += sum over the query heads of kv head h of their softmax
+ *   weight on j; other elements are left as they are.
+ *   workspace: >= nnop_paged_attention_fwd_workspace_size(...) bytes, 256-byte
+ *   aligned; calls that can overlap on the GPU need one each.
+ */
+int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_cache,
+                             const int32_t* block_table, const int32_t* lengths,
+                             float* weights, void* o, float* lse,
+                             void* workspace, size_t workspace_bytes,
+                             int64_t E, int64_t QH, int64_t KH, int64_t B,
+                             int64_t pages, int64_t page_size, int64_t max_pages,
+                             int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                             int dtype, void* stream);
+
+/*
+ * Cuts every (sequence, kv head) back to at most `budget` slots by accumulated
+ * attention weight: a sequence of at most `budget` slots keeps all of them;
+ * else its last `recent` slots stay, and of the others the budget - recent with
+ * the largest weights (equal weights: the lower slot first; -0 equals +0; NaN
+ * counts as above every number).  The kept rows of K and V are copied, in
+ * order, to slots 0, 1, ... of new_table's pages in the same pools; the pages
+ * of block_table are only read (another sequence may share them) and are the
+ * caller's to release.
+ *   new_table [B][new_max_pages] int32, budget <= new_max_pages*page_size;
+ *   its pages are distinct and none is a page that block_table names (else the
+ *   rows copied are left open).
+ *   weights [B][KH][max_pages*page_size] f32;
+ *   new_weights [B][KH][new_max_pages*page_size] f32: the kept slots' weights,
+ *   0 behind them; new_lengths [B] = min(lengths, budget);
+ *   kept [B][KH][budget] int32: the old slot of each new one, ascending, -1
+ *   behind them.  Outputs are other arrays than the inputs.
+ */
+int nnop_paged_evict(void* k_cache, void* v_cache,
+                     const int32_t* block_table, const int32_t* new_table,
+                     const int32_t* lengths, const float* weights,
+                     int32_t* new_lengths, float* new_weights, int32_t* kept,
+                     int64_t E, int64_t KH, int64_t B,
+                     int64_t pages, int64_t page_size, int64_t max_pages,
+                     int64_t new_max_pages,
+                     int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                     int64_t budget, int64_t recent, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,196 @@
+// Paged key-value cache: addressing of the page pools and the split of a ragged
+// batch over the CTAs of one launch, shared by the paged_* kernels.
+//
+// A pool is [pages][KH][page_size][E] (any strides with E contiguous); slot j of
+// sequence b lies in row j mod page_size of page table[b][j / page_size].  A table
+// entry outside [0, pages) is no page: its slots are never read or written.
+#pragma once
+
+#include "common.cuh"
+
+#include <algorithm>
+#include <utility>
+
+namespace nnop {
+namespace paged {
+
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by a multiplication (round-up method:
+// m = floor(2^32·(2^s − d)/d) + 1 with s = ceil(log2 d)).
+struct FastDiv {
+    uint32_t d = 1, m = 1;
+    int s = 0;
+    FastDiv() = default;
+    __host__ FastDiv(uint32_t div) : d(div) {
+        while (s < 31 && (1u << s) < div) ++s;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - div)) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+struct Cache {
+    const int* table;      // [B][max_pages]
+    const int* lengths;    // [B]
+    int64_t pages, max_pages;
+    int64_t page_stride, head_stride, row_stride;   // elements
+    int slots;             // max_pages · page_size, the most a sequence can hold
+    FastDiv page_size;
+
+    // Tokens sequence b has cached: its length within [0, slots].
+    __device__ __forceinline__ int length(int64_t b) const { return min(max(lengths[b], 0), slots); }
+    // Page and row of a slot (0 <= slot < slots) of sequence b; page < 0 where there is none.
+    __device__ __forceinline__ void place(const int* row_of_table, int slot, int64_t& page, int& row) const {
+        const uint32_t i = page_size.div((uint32_t)slot);
+        row = slot - (int)(i * page_size.d);
+        const int p = __ldg(row_of_table + i);
+        page = p >= 0 && p < pages ? p : -1;
+    }
+    // Element offset of a slot's row of head h; negative where there is no page.
+    __device__ __forceinline__ int64_t offset(const int* row_of_table, int slot, int64_t head_offset) const {
+        int64_t page;
+        int row;
+        place(row_of_table, slot, page, row);
+        return page < 0 ? -1 : page * page_stride + head_offset + row * row_stride;
+    }
+};
+
+// Host-side checks of what every paged entry point is given; fills `c`.
+int check_cache(const char* who, Cache& c, const int32_t* table, const int32_t* lengths, int64_t E, int64_t KH,
+                int64_t B, int64_t pages, int64_t page_size, int64_t max_pages, int64_t page_stride,
+                int64_t head_stride, int64_t row_stride, int dtype);
+
+// Runs an entry point's body; no C++ exception leaves the C ABI.
+template <typename F>
+int guarded(const char* who, F&& body) {
+    try {
+        return body();
+    } catch (...) {
+        try {
+            return fail(NNOP_ERR_ARG, std::string(who) + ": out of host memory");
+        } catch (...) {
+            return NNOP_ERR_ARG;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Split of a ragged batch.  The work of one launch is a list of units: for every
+// sequence b (in order), for every head tile h < heads, the sequence's runs of
+// kUnit slots.  CTA c of G = min(CTAs launched, units) takes units [start(c),
+// start(c + 1)), start(c) = floor(units·c / G), so all CTAs get the same number of
+// slots (to one unit) whatever the lengths are -- they live on the device, the host
+// never sees them -- and none is without a unit.  A CTA walks its units as segments:
+// consecutive units of one (b, h).
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 128;
+
+struct SplitShared {
+    long long part[kThreads / 32];
+    long long before;      // units / heads in front of sequence b
+    int b;
+};
+
+struct Split {
+    long long units;       // over all sequences and head tiles
+    long long u, u1;       // this CTA's units left
+    int G;                 // CTAs with units
+    int b, h, chunk, chunks, len;
+
+    __device__ __forceinline__ static long long start(long long units, int c, int G) { return units * c / G; }
+    // The CTA that has unit e: the largest c with start(c) <= e.
+    __device__ __forceinline__ static int owner(long long units, long long e, int G) {
+        return (int)(((e + 1) * G + units - 1) / units) - 1;
+    }
+};
+
+// Block-wide (kThreads threads): this CTA's share, set to its first unit.
+template <int kUnit>
+__device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, SplitShared& sh) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int64_t per = (B + kThreads - 1) / kThreads;
+    const int64_t b0 = min((int64_t)t * per, B), b1 = min(b0 + per, B);
+    long long mine = 0;
+    for (int64_t b = b0; b < b1; ++b) mine += (c.length(b) + kUnit - 1) / kUnit;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) sh.part[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += sh.part[w];
+        total += sh.part[w];
+    }
+    Split s;
+    s.units = total * heads;
+    s.G = (int)min((long long)gridDim.x, s.units);
+    s.u = s.u1 = 0;
+    if ((int)blockIdx.x < s.G) {
+        s.u = Split::start(s.units, blockIdx.x, s.G);
+        s.u1 = Split::start(s.units, blockIdx.x + 1, s.G);
+    }
+    if (s.u < s.u1) {
+        const long long x = s.u / heads;      // in sequence b: before(b) <= x < before(b) + chunks(b)
+        if (x >= before && x < before + mine) {
+            int64_t b = b0;
+            for (;; ++b) {
+                const int n = (c.length(b) + kUnit - 1) / kUnit;
+                if (x < before + n) break;
+                before += n;
+            }
+            sh.b = (int)b;
+            sh.before = before;
+        }
+        __syncthreads();
+        s.b = sh.b;
+        s.len = c.length(s.b);
+        s.chunks = (s.len + kUnit - 1) / kUnit;
+        const long long r = s.u - sh.before * heads;
+        s.h = (int)(r / s.chunks);
+        s.chunk = (int)(r % s.chunks);
+    }
+    return s;
+}
+
+// The next segment's (b, h) after one that ended at its last chunk.
+template <int kUnit>
+__device__ __forceinline__ void split_next(Split& s, const Cache& c, int heads) {
+    s.chunk = 0;
+    if (++s.h < heads) return;
+    s.h = 0;
+    do {
+        s.len = c.length(++s.b);
+        s.chunks = (s.len + kUnit - 1) / kUnit;
+    } while (s.chunks == 0);
+}
+
+// Launch that may start while the kernel in front of it in the stream drains; the
+// kernel calls wait_before() before it touches that kernel's results.
+template <typename... KArgs, typename... Args>
+int launch_dependent(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                     cudaStream_t s, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(NNOP_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+    }
+    return NNOP_OK;
+}
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+}  // namespace paged
+}  // namespace nnop

@@ -1,0 +1,392 @@
+// Attention of one new token per sequence over a paged key-value cache:
+//   s_j = scale·(q · k_j),  o = Σ_j softmax(s)_j v_j,  lse = log Σ_j exp(s_j)
+// over the slots j < lengths[b] that have a page, every query head of a KV head's
+// group reading the same rows.  Optionally weights[b][kv head][j] += Σ over the
+// group's heads of softmax(s)_j, which is what nnop_paged_evict goes by.
+//
+// Bound: HBM.  Each cached row is read once for all query heads of its group,
+// 2·Σ lengths·KH·E·size bytes, against 4·Σ lengths·QH·E flops.
+//
+// One launch splits the batch evenly over its CTAs whatever the lengths are
+// (paged.cuh).  A CTA runs a softmax over its part of a sequence with a running
+// maximum and sum, every warp on keys of its own, and joins its warps through
+// shared memory.  A (sequence, head tile) that lies in one CTA is written at once;
+// the others leave (maximum, sum, accumulator) in the workspace and a second launch
+// joins them.  The weights need the final lse, so the scores are kept (fp32,
+// workspace) and a third launch turns them into weights: 8 bytes per (query head,
+// slot) instead of reading K again (E·size).
+#include "paged.cuh"
+
+#include <cmath>
+
+namespace nnop {
+namespace paged {
+namespace {
+
+constexpr int kUnit = 64;          // slots per unit: 16 per warp
+constexpr int kMaxCtas = 592;      // 148 SMs × 4; the workspace is sized for it
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    void* o;
+    float *lse, *weights;
+    Cache c;
+    int64_t B;
+    int QH, KH, group, tiles;      // tiles: head tiles of R rows per KV head
+    float scale2;                  // scale · log2(e)
+    int4* join;                    // [kMaxCtas] (b, head tile, CTAs, -) of a split that starts in CTA c; CTAs = 0: none
+    float2* part_ml;               // [2·kMaxCtas][R] maximum (log2 domain), sum
+    float* part_acc;               // [2·kMaxCtas][R][E]
+    float* scores;                 // [B][QH][slots], log2 domain (with weights)
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A sequence without a single score: zeros, lse −Inf.
+template <typename T, int E>
+__device__ __forceinline__ void write_row(const AttnArgs& a, int64_t b, int qh, int e, float acc, float m, float l) {
+    const int64_t row = b * a.QH + qh;
+    static_cast<T*>(a.o)[row * E + e] = from_f<T>(l > 0.f || l != l ? acc / l : 0.f);
+    if (e == 0) a.lse[row] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// Sequences of length 0 have no unit: their rows are written here.
+template <typename T, int E>
+__device__ __forceinline__ void write_empty(const AttnArgs& a) {
+    for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x) {
+        if (a.c.length(b) != 0) continue;
+        for (int i = threadIdx.x; i < a.QH * E; i += kThreads) write_row<T, E>(a, b, i / E, i % E, 0.f, 0.f, 0.f);
+    }
+}
+
+// CUDA-core kernel: a quad of lanes per key for the scores, E/32 columns per lane
+// for the products with V; R query heads per pass over the keys.
+template <typename T, int E, int R>
+__global__ void __launch_bounds__(kThreads)
+attention_simt(AttnArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
+    constexpr int NV = E / VEC;                       // 16-byte vectors per row
+    constexpr int NQ = (NV + 3) / 4;                  // ... per lane of a quad
+    constexpr int COLS = E >= 32 ? E / 32 : 1;        // columns per lane
+    constexpr int kKeys = kUnit / 4;                  // keys per warp and unit
+    __shared__ SplitShared sh;
+    __shared__ __align__(16) float qs[R][E];
+    __shared__ float wm[4][R], wl[4][R], wacc[4][R][E];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, sub = lane & 3;
+    const int heads = a.KH * a.tiles;
+    let_next_start();
+    Split s = split_begin<kUnit>(a.c, a.B, heads, sh);
+    write_empty<T, E>(a);
+    if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
+    while (s.u < s.u1) {
+        const int c0 = s.chunk;
+        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
+        const int kvh = s.h / a.tiles, r0 = (s.h % a.tiles) * R;
+        const int rows = min(R, a.group - r0);
+        const int qh0 = kvh * a.group + r0;
+        const int* tab = a.c.table + (int64_t)s.b * a.c.max_pages;
+        const int64_t ho = (int64_t)kvh * a.c.head_stride;
+        const T* K = static_cast<const T*>(a.k);
+        const T* V = static_cast<const T*>(a.v);
+        for (int i = threadIdx.x; i < R * E; i += kThreads)
+            qs[i / E][i % E] = i / E < rows ? to_f(static_cast<const T*>(a.q)[((int64_t)s.b * a.QH + qh0) * E + i]) : 0.f;
+        __syncthreads();
+        float m[R], l[R], acc[R][COLS];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) acc[r][i] = 0.f;
+        }
+        const int end = min(s.len, c1 * kUnit);
+        for (int key0 = c0 * kUnit + warp * kKeys; key0 < end; key0 += kUnit) {
+            int64_t off[kKeys / 8];
+            float sc[kKeys / 8][R];
+#pragma unroll
+            for (int p = 0; p < kKeys / 8; ++p) {
+                const int key = key0 + p * 8 + quad;
+                off[p] = key < end ? a.c.offset(tab, key, ho) : -1;
+                float dot[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) dot[r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    const int vi = i * 4 + sub;
+                    if (off[p] >= 0 && (NV % 4 == 0 || vi < NV)) {
+                        float kv[VEC];
+                        load_vec<T, VEC>(kv, K + off[p] + vi * VEC);
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) dot[r] = fmaf(kv[e], qs[r][vi * VEC + e], dot[r]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 1);
+                    dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 2);
+                    sc[p][r] = off[p] >= 0 ? dot[r] * a.scale2 : -INFINITY;
+                    if (a.scores != nullptr && key < end && sub == 0 && r < rows)
+                        a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = sc[p][r];
+                }
+            }
+            float p[kKeys / 8][R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float mx = m[r];
+#pragma unroll
+                for (int i = 0; i < kKeys / 8; ++i) mx = fmaxf(mx, sc[i][r]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const float base = mx == -INFINITY ? 0.f : mx;      // no score yet
+                const float alpha = fast_exp2(m[r] - base);
+                m[r] = mx;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < kKeys / 8; ++i) {
+                    p[i][r] = fast_exp2(sc[i][r] - base);
+                    sum += p[i][r];
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                l[r] = l[r] * alpha + sum;
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) acc[r][i] *= alpha;
+            }
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j) {
+                const int64_t vo = __shfl_sync(0xffffffffu, off[j / 8], (j % 8) * 4);
+                float vv[COLS];
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) vv[i] = 0.f;
+                if (vo >= 0 && lane * COLS < E) load_vec<T, COLS>(vv, V + vo + lane * COLS);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float pj = __shfl_sync(0xffffffffu, p[j / 8][r], (j % 8) * 4);
+#pragma unroll
+                    for (int i = 0; i < COLS; ++i) acc[r][i] = fmaf(pj, vv[i], acc[r][i]);
+                }
+            }
+        }
+        // join the warps
+        if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                wm[warp][r] = m[r];
+                wl[warp][r] = l[r];
+            }
+        }
+        if (lane * COLS < E) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) wacc[warp][r][lane * COLS + i] = acc[r][i];
+        }
+        __syncthreads();
+        const bool whole = c0 == 0 && c1 == s.chunks;
+        const int slot = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
+        for (int i = threadIdx.x; i < rows * E; i += kThreads) {
+            const int r = i / E, e = i % E;
+            float mx = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f, ac = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = fast_exp2(wm[w][r] - base);
+                sum = fmaf(wl[w][r], f, sum);
+                ac = fmaf(wacc[w][r][e], f, ac);
+            }
+            if (whole) {
+                write_row<T, E>(a, s.b, qh0 + r, e, ac, mx, sum);
+            } else {
+                a.part_acc[((int64_t)slot * R + r) * E + e] = ac;
+                if (e == 0) a.part_ml[slot * R + r] = make_float2(mx, sum);
+            }
+        }
+        s.u += c1 - c0;
+        if (!whole && c0 == 0 && threadIdx.x == 0) {
+            const long long last = s.u + (s.chunks - c1) - 1;     // the split's last unit
+            a.join[blockIdx.x] = make_int4(s.b, s.h, Split::owner(s.units, last, s.G) - blockIdx.x + 1, 0);
+        }
+        if (s.u < s.u1) split_next<kUnit>(s, a.c, heads);
+        __syncthreads();
+    }
+}
+
+// Joins the parts of the (sequence, head tile) whose first part CTA blockIdx.x wrote;
+// blockIdx.y is the row.  Part i lies in slot 2(c + i), the first in 2c + 1.
+template <typename T, int E, int R>
+__global__ void __launch_bounds__(E) attention_join(AttnArgs a) {
+    wait_before();
+    let_next_start();
+    const int c = blockIdx.x, r = blockIdx.y, e = threadIdx.x;
+    const int4 w = a.join[c];
+    const int r0 = (w.y % a.tiles) * R;
+    if (w.z == 0 || r0 + r >= a.group) return;
+    float m = -INFINITY, l = 0.f, acc = 0.f;
+    for (int i = 0; i < w.z; ++i) {
+        const int slot = 2 * (c + i) + (i == 0 ? 1 : 0);
+        const float2 ml = a.part_ml[slot * R + r];
+        const float x = a.part_acc[((int64_t)slot * R + r) * E + e];
+        const float mx = fmaxf(m, ml.x);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float f0 = fast_exp2(m - base), f1 = fast_exp2(ml.x - base);
+        acc = acc * f0 + x * f1;
+        l = l * f0 + ml.y * f1;
+        m = mx;
+    }
+    write_row<T, E>(a, w.x, (w.y / a.tiles) * a.group + r0 + r, e, acc, m, l);
+}
+
+// weights[b][kv head][j] += Σ over the group of exp(s_j − lse).
+__global__ void __launch_bounds__(kThreads) attention_weights(AttnArgs a) {
+    __shared__ SplitShared sh;
+    wait_before();
+    Split s = split_begin<kUnit>(a.c, a.B, a.KH, sh);
+    while (s.u < s.u1) {
+        const int c0 = s.chunk;
+        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
+        const int end = min(s.len, c1 * kUnit);
+        const int64_t row0 = (int64_t)s.b * a.QH + s.h * a.group;
+        float* w = a.weights + ((int64_t)s.b * a.KH + s.h) * a.c.slots;
+        for (int j = c0 * kUnit + threadIdx.x; j < end; j += kThreads) {
+            float sum = 0.f;
+            for (int g = 0; g < a.group; ++g) {
+                const float lse2 = a.lse[row0 + g] * kLog2e;
+                sum += lse2 == -INFINITY ? 0.f : fast_exp2(a.scores[(row0 + g) * a.c.slots + j] - lse2);
+            }
+            w[j] += sum;
+        }
+        s.u += c1 - c0;
+        if (s.u < s.u1) split_next<kUnit>(s, a.c, a.KH);
+    }
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Query heads that one pass over the keys serves.
+int rows_per_tile(int64_t group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
+
+struct Layout {
+    size_t join, ml, acc, scores, bytes;
+};
+Layout layout(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t slots, bool weights) {
+    const size_t R = rows_per_tile(QH / KH);
+    Layout w;
+    w.join = 0;
+    w.ml = align256(sizeof(int4) * kMaxCtas);
+    w.acc = w.ml + align256(sizeof(float2) * 2 * kMaxCtas * R);
+    w.scores = w.acc + align256(sizeof(float) * 2 * kMaxCtas * R * E);
+    w.bytes = w.scores + (weights ? align256(sizeof(float) * (size_t)B * QH * slots) : 0);
+    return w;
+}
+
+int check_heads(int64_t E, int64_t QH, int64_t KH, int64_t B) {
+    if (E <= 0 || QH <= 0 || KH <= 0 || B < 0) return fail(NNOP_ERR_SHAPE, "paged_attention: invalid dimensions");
+    if (QH % KH != 0)
+        return fail(NNOP_ERR_SHAPE, "Number of query heads `" + std::to_string(QH) +
+                                        "` must be divisible by number of KV heads `" + std::to_string(KH) + "`.");
+    if (QH > 65535) return fail(NNOP_ERR_SHAPE, "paged_attention: too many heads");
+    return NNOP_OK;
+}
+
+template <typename T, int E, int R>
+int launch(const AttnArgs& a, cudaStream_t s) {
+    const int G = std::min(kMaxCtas, 4 * num_sms());
+    attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
+    if (const int rc = check_launch("paged_attention")) return rc;
+    if (const int rc = launch_dependent("paged_attention", attention_join<T, E, R>, dim3(G, R), dim3(E), 0, s, a))
+        return rc;
+    if (a.weights == nullptr) return NNOP_OK;
+    return launch_dependent("paged_attention", attention_weights, dim3(G), dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int E>
+int launch_rows(const AttnArgs& a, cudaStream_t s) {
+    switch (rows_per_tile(a.group)) {
+        case 1: return launch<T, E, 1>(a, s);
+        case 2: return launch<T, E, 2>(a, s);
+        case 4: return launch<T, E, 4>(a, s);
+        default: return launch<T, E, 8>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace nnop
+
+using namespace nnop;
+
+extern "C" {
+
+size_t nnop_paged_attention_fwd_workspace_size(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t page_size,
+                                               int64_t max_pages, int has_weights, int dtype) {
+    (void)dtype;
+    if (E <= 0 || QH <= 0 || KH <= 0 || B <= 0 || page_size <= 0 || max_pages < 0) return 0;
+    return paged::layout(E, QH, KH, B, page_size * max_pages, has_weights != 0).bytes;
+}
+
+int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                             const int32_t* lengths, float* weights, void* o, float* lse, void* workspace,
+                             size_t workspace_bytes, int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t pages,
+                             int64_t page_size, int64_t max_pages, int64_t page_stride, int64_t head_stride,
+                             int64_t row_stride, int dtype, void* stream) {
+    return paged::guarded("paged_attention", [&]() -> int {
+        paged::AttnArgs a{};
+        if (const int rc = paged::check_heads(E, QH, KH, B)) return rc;
+        if (const int rc = paged::check_cache("paged_attention", a.c, block_table, lengths, E, KH, B, pages, page_size,
+                                              max_pages, page_stride, head_stride, row_stride, dtype))
+            return rc;
+        if (B == 0) return NNOP_OK;
+        if (!q || !o || !lse || !workspace || (pages > 0 && (!k_cache || !v_cache)))
+            return fail(NNOP_ERR_ARG, "paged_attention: NULL pointer");
+        if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o))
+            return fail(NNOP_ERR_ALIGN, "paged_attention: tensors must be 16-byte aligned");
+        const paged::Layout w = paged::layout(E, QH, KH, B, a.c.slots, weights != nullptr);
+        if (workspace_bytes < w.bytes)
+            return fail(NNOP_ERR_WORKSPACE, "paged_attention: workspace too small (" +
+                                                std::to_string(workspace_bytes) + " < " + std::to_string(w.bytes) + ")");
+        if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+            return fail(NNOP_ERR_ALIGN, "paged_attention: workspace must be 256-byte aligned");
+        a.q = q;
+        a.k = k_cache;
+        a.v = v_cache;
+        a.o = o;
+        a.lse = lse;
+        a.weights = weights;
+        a.B = B;
+        a.QH = (int)QH;
+        a.KH = (int)KH;
+        a.group = (int)(QH / KH);
+        const int R = paged::rows_per_tile(a.group);
+        a.tiles = (a.group + R - 1) / R;
+        char* base = static_cast<char*>(workspace);
+        a.join = reinterpret_cast<int4*>(base + w.join);
+        a.part_ml = reinterpret_cast<float2*>(base + w.ml);
+        a.part_acc = reinterpret_cast<float*>(base + w.acc);
+        a.scores = weights ? reinterpret_cast<float*>(base + w.scores) : nullptr;
+        const cudaStream_t s = (cudaStream_t)stream;
+        const float sc = (float)(1.0 / std::sqrt((double)E));
+        // scale rounded to the dtype, as flash_attention has it
+        a.scale2 = paged::kLog2e * (dtype == NNOP_BF16 ? __bfloat162float(__float2bfloat16_rn(sc))
+                                    : dtype == NNOP_F16 ? __half2float(__float2half_rn(sc)) : sc);
+        NNOP_DISPATCH_DTYPE(dtype, T, {
+            switch (E) {
+                case 16: return paged::launch_rows<T, 16>(a, s);
+                case 32: return paged::launch_rows<T, 32>(a, s);
+                case 64: return paged::launch_rows<T, 64>(a, s);
+                default: return paged::launch_rows<T, 128>(a, s);
+            }
+        });
+        return NNOP_OK;
+    });
+}
+
+}  // extern "C"

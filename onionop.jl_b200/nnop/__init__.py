@@ -19,6 +19,8 @@ kpad_mask::Matrix{Bool} (KL,B) kpad_mask (B, KL) bool / uint8
 x (N, cols) [online_softmax]   x (cols, N)
 x (emb, n) [norms]             x (n, emb)
 cos, sin (E, L, B)             cos, sin (B, L, E) float32
+k_cache, v_cache (E, PS, KH, P)  k_cache, v_cache (P, KH, PS, E)
+block_table (MP, B) Int32      block_table (B, MP) int32
 position_ids (L, B)            position_ids (B, L) float32
 =============================  ===============================
 """
@@ -37,6 +39,7 @@ __all__ = [
     "add_rms_norm", "_add_rms_norm", "grad_add_rms_norm",
     "layer_norm", "_layer_norm", "grad_layer_norm",
     "llama_rope", "grad_llama_rope", "LlamaRotaryEmbedding",
+    "paged_append", "paged_append_rope", "paged_attention", "_paged_attention", "paged_evict",
     "within_gradient", "NNopError", "NNopShapeError", "lib",
 ]
 
@@ -681,3 +684,195 @@ def llama_rope(q, k, *, cos, sin):
     if within_gradient(q) or within_gradient(k):
         return _RopeFn.apply(q, k, cos, sin)
     return _llama_rope(q, k, cos, sin, bwd=False)
+
+
+# =========================================================================
+# paged key-value cache (no counterpart in the reference, whose attention takes
+# whole sequences: the step after it, one new token against the cached ones)
+# =========================================================================
+
+def _paged_dims(name, k_cache, v_cache, block_table, lengths, *others, write):
+    """Checks of the cache arguments the paged calls share; returns the device,
+    the batch and ``(pages, page_size, max_pages, strides...)`` as the C ABI
+    takes them."""
+    dev = _dev(k_cache, v_cache, block_table, lengths, *others)
+    for t in (v_cache, block_table, lengths, *others):
+        if t is not None and t.device != dev:
+            raise NNopError(-3, f"{name}: all tensors must be on one device")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise NNopShapeError(-1, f"{name}: k_cache and v_cache must be 4-d (P, KH, PS, E) of one shape")
+    if k_cache.dtype != v_cache.dtype:
+        raise NNopError(-2, f"{name}: k_cache and v_cache must share a dtype")
+    P, KH, PS, E = k_cache.shape
+    if block_table.dim() != 2 or lengths.dim() != 1 or block_table.shape[0] != lengths.shape[0]:
+        raise NNopShapeError(-1, f"{name}: block_table must be (B, MP) and lengths (B,)")
+    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise NNopError(-2, f"{name}: block_table and lengths must be int32")
+    strides = []
+    for n, sk, sv in zip((P, KH, PS), k_cache.stride(), v_cache.stride()):
+        if n > 1 and sk != sv:
+            raise NNopShapeError(-1, f"{name}: k_cache and v_cache must have the same strides")
+        if n > 1 and sk == 0 and write:
+            raise NNopShapeError(-1, f"{name}: an expanded cache cannot be written")
+        strides.append(sk if n > 1 else 0)
+    if E > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise NNopShapeError(-1, f"{name}: the caches' embedding axis must be contiguous")
+    return dev, lengths.shape[0], (P, PS, block_table.shape[1], *strides)
+
+
+def _no_grad(name, *ts):
+    if any(within_gradient(t) for t in ts):
+        raise NNopError(-3, f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _aligned(t):
+    """Contiguous and on a 16-byte boundary (a view may start off one)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _on(dev, fn, *args):
+    """Calls the library with ``dev`` as the current device and its current stream last."""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, _stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(dev)))
+
+
+def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, sin, n_new):
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, q, k, v, cos, sin, n_new, write=True)
+    _no_grad(name, q, k, v, k_cache, v_cache)
+    KH, E = k_cache.shape[1], k_cache.shape[3]
+    if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, KH, E):
+        raise NNopShapeError(-1, f"{name}: k and v must be (B, KH, T, E) = ({B}, {KH}, T, {E})")
+    if any(t is not None and t.dtype != k_cache.dtype for t in (q, k, v)):
+        raise NNopError(-2, f"{name}: q, k and v must have the dtype of the caches")
+    T = k.shape[2]
+    QH, cb, qo = 0, 1, None
+    if cos is not None:
+        cos, sin = _rope_tables(cos, sin, B, T, E)
+        cb = cos.shape[0]
+    if q is not None:
+        if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, T, E):
+            raise NNopShapeError(-1, f"{name}: q must be (B, QH, T, E) = ({B}, QH, {T}, {E})")
+        QH = q.shape[1]
+        q = _aligned(q)
+        qo = torch.empty_like(q)
+    if n_new is not None:
+        if tuple(n_new.shape) != (B,):
+            raise NNopShapeError(-1, f"{name}: n_new must be (B,) = ({B},)")
+        if n_new.dtype != torch.int32:
+            raise NNopError(-2, f"{name}: n_new must be int32")
+        n_new = n_new.contiguous()
+    k, v, lengths, block_table = _aligned(k), _aligned(v), lengths.contiguous(), block_table.contiguous()
+    new_lengths = torch.empty_like(lengths)
+    _on(dev, lib.nnop_paged_append, _ptr(q), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin), _ptr(n_new), _ptr(qo),
+        _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(lengths), _ptr(new_lengths), E, T, QH, KH, B, cb, *cache,
+        _dtype_id(k_cache))
+    return qo, new_lengths
+
+
+def paged_append(k, v, k_cache, v_cache, block_table, lengths, *, n_new=None):
+    """Writes the new rows ``k``, ``v`` (B, KH, T, E) behind what each sequence
+    has in the paged cache and returns the new lengths (B,) int32 (``lengths``
+    itself stays).
+
+    ``k_cache``, ``v_cache`` (P, KH, PS, E): the pools, written in place; any
+    strides with E contiguous, the same for both.  ``block_table`` (B, MP) int32:
+    the page of each run of PS slots; an entry outside [0, P) is no page and rows
+    meant for it are dropped, as are rows past the table's MP·PS slots.
+    ``n_new`` (B,) int32: how many of the T rows are tokens, for a padded batch
+    (default all).  A page that is written belongs to one sequence."""
+    return _paged_append("paged_append", None, k, v, k_cache, v_cache, block_table, lengths, None, None, n_new)[1]
+
+
+def paged_append_rope(q, k, v, k_cache, v_cache, block_table, lengths, *, cos, sin, n_new=None):
+    """``llama_rope(q, k; cos, sin)`` and ``paged_append`` of the rotated k in
+    one launch: returns ``(q_rot, new_lengths)``.  ``cos``, ``sin`` (B or 1, T, E)
+    float32 from ``LlamaRotaryEmbedding`` at the new tokens' positions."""
+    if cos is None or sin is None or q is None:
+        raise NNopError(-3, "paged_append_rope takes q, cos and sin")
+    return _paged_append("paged_append_rope", q, k, v, k_cache, v_cache, block_table, lengths, cos, sin, n_new)
+
+
+def _paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None):
+    """``paged_attention`` returning ``(o, lse)``, lse (B, QH, 1) float32."""
+    name = "paged_attention"
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, q, weights, write=False)
+    _no_grad(name, q, k_cache, v_cache, weights)
+    KH, E = k_cache.shape[1], k_cache.shape[3]
+    if q.dim() != 4 or q.shape[0] != B or q.shape[2] != 1:
+        raise NNopShapeError(-1, f"{name}: q must be (B, QH, 1, E) with B = {B}")
+    if q.shape[3] != E:
+        raise NNopShapeError(-1, f"Embedding dim of Q `{q.shape[3]}` must be the same as of K `{E}`.")
+    if q.dtype != k_cache.dtype:
+        raise NNopError(-2, f"{name}: q must have the dtype of the caches")
+    QH = q.shape[1]
+    if weights is not None:
+        slots = cache[1] * cache[2]
+        if tuple(weights.shape) != (B, KH, slots):
+            raise NNopShapeError(-1, f"{name}: weights must have shape (B, KH, MP·PS) = {(B, KH, slots)}")
+        if weights.dtype != torch.float32 or not weights.is_contiguous():
+            raise NNopError(-2, f"{name}: weights must be contiguous float32")
+    q, lengths, block_table = _aligned(q), lengths.contiguous(), block_table.contiguous()
+    o = torch.empty_like(q)
+    lse = torch.empty((B, QH, 1), dtype=torch.float32, device=dev)
+    dt = _dtype_id(q)
+    ws_bytes = lib.nnop_paged_attention_fwd_workspace_size(E, QH, KH, B, cache[1], cache[2], int(weights is not None), dt)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _on(dev, lib.nnop_paged_attention_fwd, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(lengths),
+        _ptr(weights), _ptr(o), _ptr(lse), _ptr(ws), ws_bytes, E, QH, KH, B, *cache, dt)
+    return o, lse
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None):
+    """Attention of one new token per sequence over the paged cache:
+    ``flash_attention`` of q (B, QH, 1, E) with the first ``lengths[b]`` slots of
+    sequence b as its keys and values; returns o (B, QH, 1, E).
+
+    Pools, table and lengths as in ``paged_append`` (slots without a page are
+    not attended to; a sequence without a slot gets zeros).  ``weights``
+    (B, KH, MP·PS) float32, contiguous: each attended slot's softmax weight,
+    summed over the query heads of its kv head, is added to it in place --
+    what ``paged_evict`` goes by."""
+    return _paged_attention(q, k_cache, v_cache, block_table, lengths, weights=weights)[0]
+
+
+def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, budget: int, recent: int = 0):
+    """Cuts each sequence's cache to at most ``budget`` slots per kv head: the
+    last ``recent`` ones and, of the others, those with the largest accumulated
+    ``weights`` (B, KH, MP·PS); equal weights: the lower slot first.  A sequence
+    of at most ``budget`` slots keeps all.
+
+    The kept rows are copied in order to the pages of ``new_table`` (B, MP')
+    int32 in the same pools; those pages are distinct and none of them is read
+    by this call.  The old pages are only read.  Returns ``(new_lengths (B,),
+    new_weights (B, KH, MP'·PS), kept (B, KH, budget))``: the kept slots' weights
+    (0 behind them) and their old slots, ascending (-1 behind them)."""
+    name = "paged_evict"
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, new_table, weights, write=True)
+    _no_grad(name, k_cache, v_cache, weights)
+    P, KH, PS, E = k_cache.shape
+    if new_table.dim() != 2 or new_table.shape[0] != B:
+        raise NNopShapeError(-1, f"{name}: new_table must be (B, MP') with B = {B}")
+    if new_table.dtype != torch.int32:
+        raise NNopError(-2, f"{name}: new_table must be int32")
+    if tuple(weights.shape) != (B, KH, cache[2] * PS):
+        raise NNopShapeError(-1, f"{name}: weights must have shape (B, KH, MP·PS) = {(B, KH, cache[2] * PS)}")
+    if weights.dtype != torch.float32:
+        raise NNopError(-2, f"{name}: weights must be float32")
+    budget, recent, slots = int(budget), int(recent), new_table.shape[1] * PS
+    if not 0 <= recent <= budget <= slots:
+        raise NNopShapeError(-1, f"{name}: 0 <= recent ({recent}) <= budget ({budget}) <= slots of new_table ({slots})")
+    lengths, weights = lengths.contiguous(), weights.contiguous()
+    block_table, new_table = block_table.contiguous(), new_table.contiguous()
+    new_lengths = torch.empty_like(lengths)
+    new_weights = torch.empty((B, KH, slots), dtype=torch.float32, device=dev)
+    kept = torch.empty((B, KH, budget), dtype=torch.int32, device=dev)
+    _on(dev, lib.nnop_paged_evict, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(new_table), _ptr(lengths),
+        _ptr(weights), _ptr(new_lengths), _ptr(new_weights), _ptr(kept), E, KH, B, *cache[:3], new_table.shape[1],
+        *cache[3:], budget, recent, _dtype_id(k_cache))
+    return new_lengths, new_weights, kept

@@ -66,6 +66,10 @@ SIGNATURES = {
     "nnop_layer_norm_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _int, _vp]),
     "nnop_llama_rope": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f, _int, _vp]),
     "nnop_llama_rope_cos_sin": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "nnop_paged_append": (_int, [_vp] * 12 + [_i64] * 12 + [_int, _vp]),
+    "nnop_paged_attention_fwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
+    "nnop_paged_attention_fwd": (_int, [_vp] * 9 + [_sz] + [_i64] * 10 + [_int, _vp]),
+    "nnop_paged_evict": (_int, [_vp] * 9 + [_i64] * 12 + [_int, _vp]),
 }
 
 

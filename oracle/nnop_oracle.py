@@ -359,3 +359,95 @@ def rope_bwd(dq, dk, cos, sin):
     """``∇llama_rope`` = the same kernel with ``sin_sign = -1``
     (``src/rope/llama_rope.jl:86,92``)."""
     return _rope(dq, cos, sin, -1.0), _rope(dk, cos, sin, -1.0)
+
+
+# ---------------------------------------------------------------------------
+# paged key-value cache (pools (P, KH, PS, E), table (B, MP), slots in order)
+# ---------------------------------------------------------------------------
+
+def paged_places(table, b, slots, pages, page_size):
+    """``(page, row)`` of slots of sequence b; page -1 where the table names none."""
+    slots = np.asarray(slots, np.int64)
+    page = np.asarray(table, np.int64)[b, slots // page_size] if slots.size else slots
+    return np.where((page >= 0) & (page < pages), page, -1), slots % page_size
+
+
+def paged_length(lengths, b, table, page_size):
+    return int(min(max(int(lengths[b]), 0), table.shape[1] * page_size))
+
+
+def paged_append(k, v, k_cache, v_cache, table, lengths, n_new=None):
+    """New rows (B, KH, T, E) behind each sequence's slots: ``(k_cache, v_cache,
+    new_lengths)``, the pools as copies."""
+    k_cache, v_cache = k_cache.copy(), v_cache.copy()
+    P, PS = k_cache.shape[0], k_cache.shape[2]
+    B, _, T, _ = k.shape
+    slots = table.shape[1] * PS
+    new_lengths = np.zeros(B, np.int32)
+    for b in range(B):
+        n = paged_length(lengths, b, table, PS)
+        add = T if n_new is None else min(max(int(n_new[b]), 0), T)
+        new_lengths[b] = min(n + add, slots)
+        for t in range(new_lengths[b] - n):
+            (page,), (row,) = paged_places(table, b, [n + t], P, PS)
+            if page >= 0:
+                k_cache[page, :, row], v_cache[page, :, row] = k[b, :, t], v[b, :, t]
+    return k_cache, v_cache, new_lengths
+
+
+def paged_attention(q, k_cache, v_cache, table, lengths, *, scale):
+    """One new token q (B, QH, 1, E) per sequence over its cached slots:
+    ``(o, lse, w)`` with w (B, KH, MP·PS) the softmax weights summed over each kv
+    head's query heads; a sequence without a slot has o = 0, lse = -Inf."""
+    B, QH, _, E = q.shape
+    P, KH, PS, _ = k_cache.shape
+    G = QH // KH
+    q = np.asarray(q, np.float64).reshape(B, KH, G, E)
+    o, lse = np.zeros((B, KH, G, E)), np.full((B, KH, G), -np.inf)
+    w = np.zeros((B, KH, table.shape[1] * PS))
+    for b in range(B):
+        slots = np.arange(paged_length(lengths, b, table, PS))
+        page, row = paged_places(table, b, slots, P, PS)
+        slots, page, row = (x[page >= 0] for x in (slots, page, row))
+        if not slots.size:
+            continue
+        k = np.asarray(k_cache[page, :, row], np.float64)       # (n, KH, E)
+        v = np.asarray(v_cache[page, :, row], np.float64)
+        s = np.einsum("hge,nhe->hgn", q[b], k) * scale
+        m = s.max(-1, keepdims=True)
+        p = np.exp(s - m)
+        l = p.sum(-1, keepdims=True)
+        p /= l
+        o[b] = np.einsum("hgn,nhe->hge", p, v)
+        lse[b] = (m + np.log(l))[..., 0]
+        w[b][:, slots] = p.sum(1)
+    return o.reshape(B, QH, 1, E), lse.reshape(B, QH, 1), w
+
+
+def paged_evict(k_cache, v_cache, table, new_table, lengths, weights, *, budget, recent):
+    """``(k_cache, v_cache, new_lengths, new_weights, kept)``, the pools as copies:
+    per (sequence, kv head) the last ``recent`` slots and the heaviest of the
+    others (NaN above all, equal weights by rising slot), ``budget`` in all."""
+    src_k, src_v = k_cache, v_cache
+    k_cache, v_cache = k_cache.copy(), v_cache.copy()
+    P, KH, PS, _ = k_cache.shape
+    B = table.shape[0]
+    new_lengths = np.zeros(B, np.int32)
+    new_weights = np.zeros((B, KH, new_table.shape[1] * PS), np.float32)
+    kept = np.full((B, KH, budget), -1, np.int32)
+    for b in range(B):
+        n = paged_length(lengths, b, table, PS)
+        count = new_lengths[b] = min(n, budget)
+        last = n if n <= budget else recent
+        for h in range(KH):
+            w = weights[b, h, :n - last].astype(np.float64)
+            order = sorted(range(n - last), key=lambda i: (not np.isnan(w[i]), 0.0 if np.isnan(w[i]) else -w[i], i))
+            keep = np.array(sorted(order[:count - last]) + list(range(n - last, n)), np.int64)
+            kept[b, h, :count] = keep
+            new_weights[b, h, :count] = weights[b, h, keep]
+            page, row = paged_places(table, b, keep, P, PS)
+            to, at = paged_places(new_table, b, np.arange(count), P, PS)
+            ok = (page >= 0) & (to >= 0)
+            k_cache[to[ok], h, at[ok]] = src_k[page[ok], h, row[ok]]
+            v_cache[to[ok], h, at[ok]] = src_v[page[ok], h, row[ok]]
+    return k_cache, v_cache, new_lengths, new_weights, kept
