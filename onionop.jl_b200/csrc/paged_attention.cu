@@ -18,6 +18,7 @@
 #include "paged.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace nnop {
 namespace paged {
@@ -220,6 +221,314 @@ attention_simt(AttnArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Tensor-core kernel for the 16-bit types (mma.sync m16n8k16).  The op is bound by
+// HBM: at 8 query heads a key row it needs 1/6 of mma.sync's rate, so what matters
+// is that the loads never stop, and the operands go from global memory straight
+// into the fragments -- no shared memory, no barrier, every warp on its own keys:
+//
+//   Sᵀ (16 keys × 8 heads) = K (A: 16 × E) · Qᵀ (B: E × 8)
+//   Oᵀ (E × 8 heads)      += Vᵀ (A: E × 16 keys) · Pᵀ (B: 16 keys × 8)
+//
+// with keys (then E) on the side of 16 and the group's heads on the side of 8, so a
+// group of up to 8 heads wastes nothing.  A sum over E may run in any order, so a
+// lane's A fragments of two k16 steps are the 16 consecutive bytes it loads of a K
+// row (4 lanes read 64 bytes of each of 8 rows), and Q is laid out to match.  The
+// rows of Oᵀ may be any E order too: a lane loads 16 bytes of 4 V rows (8 lanes read
+// 128 bytes of a row) and pairs two keys' halves by byte permutes.  Sᵀ's
+// accumulators become Pᵀ's B fragments by movmatrix.  P goes in as the sum of two
+// 16-bit terms: rounded once to 16 bits it would cost as much accuracy as rounding
+// the result does.  f16: P is scaled by 2^14, which the running sum shares, so that
+// weights down to 2^-38 of the largest count.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
+
+// W words of a row that is read once, zeros without a page.
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&r)[W], const void* p, bool live) {
+    const int on = live;
+    if constexpr (W == 4) {
+        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+                     " @p ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];\n}"
+                     : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]) : "l"(p), "r"(on));
+    } else if constexpr (W == 2) {
+        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n @p ld.global.nc.v2.b32 {%0,%1}, [%2];\n}"
+                     : "=&r"(r[0]), "=&r"(r[1]) : "l"(p), "r"(on));
+    } else {
+        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.nc.b32 %0, [%1];\n}"
+                     : "=&r"(r[0]) : "l"(p), "r"(on));
+    }
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi, float& rest_lo, float& rest_hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        rest_lo = lo - __low2float(h);
+        rest_hi = hi - __high2float(h);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        rest_lo = lo - __low2float(h);
+        rest_hi = hi - __high2float(h);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+template <int E> struct MmaShape {
+    static constexpr int kTiles = E >= 128 ? 1 : E == 64 ? 2 : 4;   // 16-key tiles a warp takes at once (8 KB of K and V from E = 32)
+    static constexpr int kKeys = 16 * kTiles;
+    static constexpr int kUnit = 4 * kKeys;                         // slots per unit
+};
+
+// WT: head tiles (of 8) per CTA.  The warps of one key group share the K and V rows
+// they read (by L1), those of one head tile share the keys out.
+template <typename T, int E, int WT>
+__global__ void __launch_bounds__(kThreads, 3)
+attention_mma(AttnArgs a) {
+    using S = MmaShape<E>;
+    constexpr int R = 8 * WT;
+    constexpr int KW = E >= 32 ? 4 : 2, KC = E / (8 * KW);     // words per K load, loads per row
+    constexpr int VW = E >= 64 ? 4 : E == 32 ? 2 : 1, VC = E / (16 * VW);
+    constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
+    __shared__ SplitShared sh;
+    __shared__ float wm[4][8], wl[4][8];
+    __shared__ __align__(16) float wacc[4][8][E];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, sub = lane & 3;
+    const int tile = warp % WT, part = warp / WT;
+    const int heads = a.KH * a.tiles;
+    const T* K = static_cast<const T*>(a.k);
+    const T* V = static_cast<const T*>(a.v);
+    let_next_start();
+    Split s = split_begin<S::kUnit>(a.c, a.B, heads, sh);
+    write_empty<T, E>(a);
+    if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
+    while (s.u < s.u1) {
+        const int c0 = s.chunk;
+        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
+        const int kvh = s.h / a.tiles, r0 = (s.h % a.tiles) * R;
+        const int rows = min(R, a.group - r0);
+        const int qh0 = kvh * a.group + r0;
+        const int* tab = a.c.table + (int64_t)s.b * a.c.max_pages;
+        const int64_t ho = (int64_t)kvh * a.c.head_stride;
+        // Q: B fragments of all k16 steps; head gid of this warp's tile
+        uint32_t q[KC][KW];
+        {
+            const int r = tile * 8 + gid;
+            const T* row = static_cast<const T*>(a.q) + ((int64_t)s.b * a.QH + qh0 + r) * E;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) load_words<KW>(q[c], row + (c * 4 + sub) * (2 * KW), r < rows);
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float acc[VC][VW][4];
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[c][j][i] = 0.f;
+        const int end = min(s.len, c1 * S::kUnit);
+        constexpr int kStep = S::kKeys * (4 / WT);
+        constexpr int NO = S::kKeys > 32 ? 2 : 1;
+        uint32_t kr[S::kTiles][2][KC][KW], vr[S::kTiles][4][VC][VW];
+        int64_t off[NO], next[NO];
+        // offsets of a step's keys: key i in lane i mod 32
+        auto find = [&](int64_t (&o)[NO], int key0) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i) {
+                const int key = key0 + i * 32 + (S::kKeys < 32 ? (lane & 15) : lane);
+                o[i] = key < end ? a.c.offset(tab, key, ho) : -1;
+            }
+        };
+        auto load_k = [&](const int64_t (&o)[NO]) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = t * 16 + i * 8;
+                    const int64_t x = __shfl_sync(0xffffffffu, o[at / 32], at % 32 + gid);
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], K + x + (c * 4 + sub) * (2 * KW), x >= 0);
+                }
+        };
+        auto load_v = [&](const int64_t (&o)[NO]) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = t * 16 + (i >> 1) * 8 + (i & 1);
+                    const int64_t x = __shfl_sync(0xffffffffu, o[at / 32], at % 32 + 2 * sub);
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], V + x + (c * 8 + gid) * (2 * VW), x >= 0);
+                }
+        };
+        int key0 = c0 * S::kUnit + part * S::kKeys;
+        if (key0 < end) {
+            find(off, key0);
+            load_k(off);
+            load_v(off);
+            find(next, key0 + kStep);
+        }
+        for (; key0 < end; key0 += kStep) {
+            float d[S::kTiles][4];
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int w = 0; w < KW; w += 2)
+                        mma16816<T>(d[t], kr[t][0][c][w], kr[t][1][c][w], kr[t][0][c][w + 1], kr[t][1][c][w + 1], q[c][w],
+                                    q[c][w + 1]);
+            }
+            const bool more = key0 + kStep < end;
+            if (more) load_k(next);
+            // scores to weights against the running maximum; heads 2·sub and 2·sub + 1
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = t * 16 + i * 8;
+                    const bool live = __shfl_sync(0xffffffffu, off[at / 32], at % 32 + gid) >= 0;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float& x = d[t][i * 2 + j];
+                        x = live ? x * a.scale2 : -INFINITY;
+                        mx[j] = fmaxf(mx[j], x);
+                        const int key = key0 + at + gid, r = tile * 8 + 2 * sub + j;
+                        if (a.scores != nullptr && key < end && r < rows)
+                            a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = x;
+                    }
+                }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+            }
+            float base[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) base[j] = mx[j] == -INFINITY ? 0.f : mx[j] - kShift;    // -Inf: no score yet
+            if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+                const float f0 = fast_exp2(m[0] - kShift - base[0]), f1 = fast_exp2(m[1] - kShift - base[1]);
+                l[0] *= f0;
+                l[1] *= f1;
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) {
+                        acc[c][j][0] *= f0;
+                        acc[c][j][1] *= f1;
+                        acc[c][j][2] *= f0;
+                        acc[c][j][3] *= f1;
+                    }
+                m[0] = mx[0];
+                m[1] = mx[1];
+            }
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) {
+                uint32_t b[2][2];      // [16-bit term][key half]
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float p0 = fast_exp2(d[t][i * 2] - base[0]), p1 = fast_exp2(d[t][i * 2 + 1] - base[1]);
+                    l[0] += p0;
+                    l[1] += p1;
+                    float e0, e1, u0, u1;
+                    b[0][i] = transpose8x8(pack2<T>(p0, p1, e0, e1));
+                    b[1][i] = transpose8x8(pack2<T>(e0, e1, u0, u1));
+                }
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) {
+                        const uint32_t a0 = __byte_perm(vr[t][0][c][j], vr[t][1][c][j], 0x5410);
+                        const uint32_t a1 = __byte_perm(vr[t][0][c][j], vr[t][1][c][j], 0x7632);
+                        const uint32_t a2 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x5410);
+                        const uint32_t a3 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x7632);
+                        mma16816<T>(acc[c][j], a0, a1, a2, a3, b[0][0], b[0][1]);
+                        mma16816<T>(acc[c][j], a0, a1, a2, a3, b[1][0], b[1][1]);
+                    }
+            }
+            if (more) load_v(next);
+#pragma unroll
+            for (int i = 0; i < NO; ++i) off[i] = next[i];
+            find(next, key0 + 2 * kStep);
+        }
+        // join the warps of each head tile
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+        }
+        if (gid == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                wm[warp][2 * sub + j] = m[j] - kShift;
+                wl[warp][2 * sub + j] = l[j];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < VW; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float2*>(&wacc[warp][2 * sub + h][(c * 8 + gid) * (2 * VW) + 2 * j]) =
+                        make_float2(acc[c][j][h], acc[c][j][2 + h]);
+        __syncthreads();
+        const bool whole = c0 == 0 && c1 == s.chunks;
+        const int slot = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
+        for (int i = threadIdx.x; i < rows * E; i += kThreads) {
+            const int r = i / E, e = i % E;
+            float mw[4 / WT], mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4 / WT; ++w) {
+                mw[w] = wm[w * WT + r / 8][r % 8];
+                mx = fmaxf(mx, mw[w]);
+            }
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f, ac = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4 / WT; ++w) {
+                const float f = fast_exp2(mw[w] - base);
+                sum = fmaf(wl[w * WT + r / 8][r % 8], f, sum);
+                ac = fmaf(wacc[w * WT + r / 8][r % 8][e], f, ac);
+            }
+            if (whole) {
+                write_row<T, E>(a, s.b, qh0 + r, e, ac, mx, sum);
+            } else {
+                a.part_acc[((int64_t)slot * R + r) * E + e] = ac;
+                if (e == 0) a.part_ml[slot * R + r] = make_float2(mx, sum);
+            }
+        }
+        s.u += c1 - c0;
+        if (!whole && c0 == 0 && threadIdx.x == 0) {
+            const long long last = s.u + (s.chunks - c1) - 1;     // the split's last unit
+            a.join[blockIdx.x] = make_int4(s.b, s.h, Split::owner(s.units, last, s.G) - blockIdx.x + 1, 0);
+        }
+        if (s.u < s.u1) split_next<S::kUnit>(s, a.c, heads);
+        __syncthreads();
+    }
+}
+
 // Joins the parts of the (sequence, head tile) whose first part CTA blockIdx.x wrote;
 // blockIdx.y is the row.  Part i lies in slot 2(c + i), the first in 2c + 1.
 template <typename T, int E, int R>
@@ -272,13 +581,16 @@ __global__ void __launch_bounds__(kThreads) attention_weights(AttnArgs a) {
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Query heads that one pass over the keys serves.
-int rows_per_tile(int64_t group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
+int rows_per_tile(int64_t group, int dtype) {
+    if (dtype != NNOP_F32) return group <= 8 ? 8 : group <= 16 ? 16 : 32;
+    return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
+}
 
 struct Layout {
     size_t join, ml, acc, scores, bytes;
 };
-Layout layout(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t slots, bool weights) {
-    const size_t R = rows_per_tile(QH / KH);
+Layout layout(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t slots, bool weights, int dtype) {
+    const size_t R = rows_per_tile(QH / KH, dtype);
     Layout w;
     w.join = 0;
     w.ml = align256(sizeof(int4) * kMaxCtas);
@@ -299,8 +611,14 @@ int check_heads(int64_t E, int64_t QH, int64_t KH, int64_t B) {
 
 template <typename T, int E, int R>
 int launch(const AttnArgs& a, cudaStream_t s) {
-    const int G = std::min(kMaxCtas, 4 * num_sms());
-    attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
+    int G;
+    if constexpr (std::is_same<T, float>::value) {
+        G = std::min(kMaxCtas, 4 * num_sms());
+        attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
+    } else {
+        G = std::min(kMaxCtas, 3 * num_sms());
+        attention_mma<T, E, R / 8><<<G, kThreads, 0, s>>>(a);
+    }
     if (const int rc = check_launch("paged_attention")) return rc;
     if (const int rc = launch_dependent("paged_attention", attention_join<T, E, R>, dim3(G, R), dim3(E), 0, s, a))
         return rc;
@@ -309,12 +627,20 @@ int launch(const AttnArgs& a, cudaStream_t s) {
 }
 
 template <typename T, int E>
-int launch_rows(const AttnArgs& a, cudaStream_t s) {
-    switch (rows_per_tile(a.group)) {
-        case 1: return launch<T, E, 1>(a, s);
-        case 2: return launch<T, E, 2>(a, s);
-        case 4: return launch<T, E, 4>(a, s);
-        default: return launch<T, E, 8>(a, s);
+int launch_rows(const AttnArgs& a, int rows, cudaStream_t s) {
+    if constexpr (std::is_same<T, float>::value) {
+        switch (rows) {
+            case 1: return launch<T, E, 1>(a, s);
+            case 2: return launch<T, E, 2>(a, s);
+            case 4: return launch<T, E, 4>(a, s);
+            default: return launch<T, E, 8>(a, s);
+        }
+    } else {
+        switch (rows) {
+            case 8: return launch<T, E, 8>(a, s);
+            case 16: return launch<T, E, 16>(a, s);
+            default: return launch<T, E, 32>(a, s);
+        }
     }
 }
 
@@ -328,9 +654,8 @@ extern "C" {
 
 size_t nnop_paged_attention_fwd_workspace_size(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t page_size,
                                                int64_t max_pages, int has_weights, int dtype) {
-    (void)dtype;
     if (E <= 0 || QH <= 0 || KH <= 0 || B <= 0 || page_size <= 0 || max_pages < 0) return 0;
-    return paged::layout(E, QH, KH, B, page_size * max_pages, has_weights != 0).bytes;
+    return paged::layout(E, QH, KH, B, page_size * max_pages, has_weights != 0, dtype).bytes;
 }
 
 int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -349,7 +674,7 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
             return fail(NNOP_ERR_ARG, "paged_attention: NULL pointer");
         if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o))
             return fail(NNOP_ERR_ALIGN, "paged_attention: tensors must be 16-byte aligned");
-        const paged::Layout w = paged::layout(E, QH, KH, B, a.c.slots, weights != nullptr);
+        const paged::Layout w = paged::layout(E, QH, KH, B, a.c.slots, weights != nullptr, dtype);
         if (workspace_bytes < w.bytes)
             return fail(NNOP_ERR_WORKSPACE, "paged_attention: workspace too small (" +
                                                 std::to_string(workspace_bytes) + " < " + std::to_string(w.bytes) + ")");
@@ -365,7 +690,7 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
         a.QH = (int)QH;
         a.KH = (int)KH;
         a.group = (int)(QH / KH);
-        const int R = paged::rows_per_tile(a.group);
+        const int R = paged::rows_per_tile(a.group, dtype);
         a.tiles = (a.group + R - 1) / R;
         char* base = static_cast<char*>(workspace);
         a.join = reinterpret_cast<int4*>(base + w.join);
@@ -379,10 +704,10 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
                                     : dtype == NNOP_F16 ? __half2float(__float2half_rn(sc)) : sc);
         NNOP_DISPATCH_DTYPE(dtype, T, {
             switch (E) {
-                case 16: return paged::launch_rows<T, 16>(a, s);
-                case 32: return paged::launch_rows<T, 32>(a, s);
-                case 64: return paged::launch_rows<T, 64>(a, s);
-                default: return paged::launch_rows<T, 128>(a, s);
+                case 16: return paged::launch_rows<T, 16>(a, R, s);
+                case 32: return paged::launch_rows<T, 32>(a, R, s);
+                case 64: return paged::launch_rows<T, 64>(a, R, s);
+                default: return paged::launch_rows<T, 128>(a, R, s);
             }
         });
         return NNOP_OK;

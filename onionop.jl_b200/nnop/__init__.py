@@ -691,37 +691,43 @@ def llama_rope(q, k, *, cos, sin):
 # whole sequences: the step after it, one new token against the cached ones)
 # =========================================================================
 
-def _paged_dims(name, k_cache, v_cache, block_table, lengths, *others, write):
-    """Checks of the cache arguments the paged calls share; returns the device,
-    the batch and ``(pages, page_size, max_pages, strides...)`` as the C ABI
+# These run once per generated token, where the host's time counts: plain checks, and
+# the device as its index (-1 on the CPU).
+
+def _paged_dims(name, k_cache, v_cache, block_table, lengths, others, write):
+    """Checks of the cache arguments the paged calls share; returns the device's
+    index, the batch and ``(pages, page_size, max_pages, strides...)`` as the C ABI
     takes them."""
-    dev = _dev(k_cache, v_cache, block_table, lengths, *others)
-    for t in (v_cache, block_table, lengths, *others):
-        if t is not None and t.device != dev:
+    dev = k_cache.get_device()
+    for t in (k_cache, v_cache, block_table, lengths, *others):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            if not (k_cache.is_cuda and t.is_cuda):
+                raise NNopError(-3, "nnop operates on CUDA tensors only (no CPU fallback)")
             raise NNopError(-3, f"{name}: all tensors must be on one device")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
         raise NNopShapeError(-1, f"{name}: k_cache and v_cache must be 4-d (P, KH, PS, E) of one shape")
     if k_cache.dtype != v_cache.dtype:
         raise NNopError(-2, f"{name}: k_cache and v_cache must share a dtype")
-    P, KH, PS, E = k_cache.shape
-    if block_table.dim() != 2 or lengths.dim() != 1 or block_table.shape[0] != lengths.shape[0]:
+    tshape, nshape = block_table.shape, lengths.shape
+    if len(tshape) != 2 or len(nshape) != 1 or tshape[0] != nshape[0]:
         raise NNopShapeError(-1, f"{name}: block_table must be (B, MP) and lengths (B,)")
     if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise NNopError(-2, f"{name}: block_table and lengths must be int32")
-    strides = []
-    for n, sk, sv in zip((P, KH, PS), k_cache.stride(), v_cache.stride()):
-        if n > 1 and sk != sv:
+    strides = k_cache.stride()
+    if min(shape) <= 1 or strides != v_cache.stride():     # the stride of an axis of length 1 means nothing
+        strides, sv = (tuple(st if n > 1 else 0 for n, st in zip(shape, t.stride())) for t in (k_cache, v_cache))
+        if strides[:3] != sv[:3]:
             raise NNopShapeError(-1, f"{name}: k_cache and v_cache must have the same strides")
-        if n > 1 and sk == 0 and write:
-            raise NNopShapeError(-1, f"{name}: an expanded cache cannot be written")
-        strides.append(sk if n > 1 else 0)
-    if E > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+    if shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
         raise NNopShapeError(-1, f"{name}: the caches' embedding axis must be contiguous")
-    return dev, lengths.shape[0], (P, PS, block_table.shape[1], *strides)
+    if write and any(st == 0 and n > 1 for n, st in zip(shape, strides)):
+        raise NNopShapeError(-1, f"{name}: an expanded cache cannot be written")
+    return dev, nshape[0], (shape[0], shape[2], tshape[1], strides[0], strides[1], strides[2])
 
 
 def _no_grad(name, *ts):
-    if any(within_gradient(t) for t in ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise NNopError(-3, f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -734,16 +740,16 @@ def _aligned(t):
 
 
 def _on(dev, fn, *args):
-    """Calls the library with ``dev`` as the current device and its current stream last."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, _stream(dev)))
+    """Calls the library on device ``dev`` with its current stream last."""
+    if dev == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, _stream(dev)))
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, sin, n_new):
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, q, k, v, cos, sin, n_new, write=True)
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (q, k, v, cos, sin, n_new), True)
     _no_grad(name, q, k, v, k_cache, v_cache)
     KH, E = k_cache.shape[1], k_cache.shape[3]
     if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, KH, E):
@@ -801,30 +807,29 @@ def paged_append_rope(q, k, v, k_cache, v_cache, block_table, lengths, *, cos, s
 def _paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None):
     """``paged_attention`` returning ``(o, lse)``, lse (B, QH, 1) float32."""
     name = "paged_attention"
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, q, weights, write=False)
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (q, weights), False)
     _no_grad(name, q, k_cache, v_cache, weights)
     KH, E = k_cache.shape[1], k_cache.shape[3]
-    if q.dim() != 4 or q.shape[0] != B or q.shape[2] != 1:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[2] != 1:
         raise NNopShapeError(-1, f"{name}: q must be (B, QH, 1, E) with B = {B}")
-    if q.shape[3] != E:
-        raise NNopShapeError(-1, f"Embedding dim of Q `{q.shape[3]}` must be the same as of K `{E}`.")
+    if shape[3] != E:
+        raise NNopShapeError(-1, f"Embedding dim of Q `{shape[3]}` must be the same as of K `{E}`.")
     if q.dtype != k_cache.dtype:
         raise NNopError(-2, f"{name}: q must have the dtype of the caches")
-    QH = q.shape[1]
+    QH = shape[1]
     if weights is not None:
-        slots = cache[1] * cache[2]
-        if tuple(weights.shape) != (B, KH, slots):
-            raise NNopShapeError(-1, f"{name}: weights must have shape (B, KH, MP·PS) = {(B, KH, slots)}")
+        if tuple(weights.shape) != (B, KH, cache[1] * cache[2]):
+            raise NNopShapeError(-1, f"{name}: weights must have shape (B, KH, MP·PS) = {(B, KH, cache[1] * cache[2])}")
         if weights.dtype != torch.float32 or not weights.is_contiguous():
             raise NNopError(-2, f"{name}: weights must be contiguous float32")
     q, lengths, block_table = _aligned(q), lengths.contiguous(), block_table.contiguous()
-    o = torch.empty_like(q)
-    lse = torch.empty((B, QH, 1), dtype=torch.float32, device=dev)
-    dt = _dtype_id(q)
-    ws_bytes = lib.nnop_paged_attention_fwd_workspace_size(E, QH, KH, B, cache[1], cache[2], int(weights is not None), dt)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _on(dev, lib.nnop_paged_attention_fwd, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(lengths),
-        _ptr(weights), _ptr(o), _ptr(lse), _ptr(ws), ws_bytes, E, QH, KH, B, *cache, dt)
+    dt, weigh = _dtype_id(q), weights is not None
+    ws_bytes = lib.nnop_paged_attention_fwd_workspace_size(E, QH, KH, B, cache[1], cache[2], weigh, dt)
+    o, lse = torch.empty_like(q), q.new_empty((B, QH, 1), dtype=torch.float32)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
+    _on(dev, lib.nnop_paged_attention_fwd, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+        lengths.data_ptr(), _ptr(weights), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, E, QH, KH, B, *cache, dt)
     return o, lse
 
 
@@ -853,7 +858,7 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
     new_weights (B, KH, MP'·PS), kept (B, KH, budget))``: the kept slots' weights
     (0 behind them) and their old slots, ascending (-1 behind them)."""
     name = "paged_evict"
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, new_table, weights, write=True)
+    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (new_table, weights), True)
     _no_grad(name, k_cache, v_cache, weights)
     P, KH, PS, E = k_cache.shape
     if new_table.dim() != 2 or new_table.shape[0] != B:
@@ -870,8 +875,7 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
     lengths, weights = lengths.contiguous(), weights.contiguous()
     block_table, new_table = block_table.contiguous(), new_table.contiguous()
     new_lengths = torch.empty_like(lengths)
-    new_weights = torch.empty((B, KH, slots), dtype=torch.float32, device=dev)
-    kept = torch.empty((B, KH, budget), dtype=torch.int32, device=dev)
+    new_weights, kept = weights.new_empty((B, KH, slots)), lengths.new_empty((B, KH, budget))
     _on(dev, lib.nnop_paged_evict, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(new_table), _ptr(lengths),
         _ptr(weights), _ptr(new_lengths), _ptr(new_weights), _ptr(kept), E, KH, B, *cache[:3], new_table.shape[1],
         *cache[3:], budget, recent, _dtype_id(k_cache))
