@@ -74,17 +74,23 @@ int guarded(const char* who, F&& body) {
 
 // ---------------------------------------------------------------------------
 // Split of a ragged batch.  The work of one launch is a list of units: for every
-// sequence b (in order), for every head tile h < heads, the sequence's runs of
-// kUnit slots.  CTA c of G = min(CTAs launched, units) takes units [start(c),
+// sequence b (in order), for every head tile h < heads, the sequence's chunks of
+// `unit` slots.  CTA c of G = min(CTAs launched, units) takes units [start(c),
 // start(c + 1)), start(c) = floor(units·c / G), so all CTAs get the same number of
-// slots (to one unit) whatever the lengths are -- they live on the device, the host
-// never sees them -- and none is without a unit.  A CTA walks its units as segments:
-// consecutive units of one (b, h).
+// units (to one) whatever the lengths are -- they live on the device, the host never
+// sees them -- and none is without one.  A CTA walks its units as segments:
+// consecutive chunks of one (b, h).
+//
+// To begin and end a segment costs a CTA about what the slots of one chunk cost, so
+// where CTAs have several units each, every (b, h) counts one chunk more, an empty
+// one in front (`extra`).  Sequences of 1 to 8192 tokens, 64 of them: the slowest CTA
+// finished 17 us after the median of 157 without it (attention_mma, B200).
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 128;
 
 struct SplitShared {
-    long long part[kThreads / 32];
+    long long slots[kThreads / 32];
+    int some[kThreads / 32];
     long long before;      // units / heads in front of sequence b
     int b;
 };
@@ -93,40 +99,73 @@ struct Split {
     long long units;       // over all sequences and head tiles
     long long u, u1;       // this CTA's units left
     int G;                 // CTAs with units
+    int extra;
     int b, h, chunk, chunks, len;
+    long long before;      // units / heads in front of sequence b
 
     __device__ __forceinline__ static long long start(long long units, int c, int G) { return units * c / G; }
     // The CTA that has unit e: the largest c with start(c) <= e.
     __device__ __forceinline__ static int owner(long long units, long long e, int G) {
         return (int)(((e + 1) * G + units - 1) / units) - 1;
     }
+    template <int kUnit>
+    __device__ __forceinline__ int chunks_of(int n) const {
+        return n == 0 ? 0 : (n + kUnit - 1) / kUnit + extra;
+    }
+    // Slots [first, last) of chunks c0 to c1 - 1 of this sequence.
+    template <int kUnit>
+    __device__ __forceinline__ int first_slot(int c0) const { return max(c0 - extra, 0) * kUnit; }
+    template <int kUnit>
+    __device__ __forceinline__ int end_slot(int c1) const { return min(len, (c1 - extra) * kUnit); }
 };
 
-// Block-wide (kThreads threads): this CTA's share, set to its first unit.
+// Block-wide (kThreads threads): this CTA's share, set to its first unit.  The units
+// are counted as `heads` head tiles and `ctas` CTAs make them.
 template <int kUnit>
-__device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, SplitShared& sh) {
+__device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, int ctas, SplitShared& sh) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t per = (B + kThreads - 1) / kThreads;
     const int64_t b0 = min((int64_t)t * per, B), b1 = min(b0 + per, B);
     long long mine = 0;
-    for (int64_t b = b0; b < b1; ++b) mine += (c.length(b) + kUnit - 1) / kUnit;
+    int some = 0;              // sequences with slots
+    for (int64_t b = b0; b < b1; ++b) {
+        const int n = c.length(b);
+        mine += (n + kUnit - 1) / kUnit;
+        some += n > 0;
+    }
     long long incl = mine;
+    int incl_some = some;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+        const int up_some = __shfl_up_sync(0xffffffffu, incl_some, o);
+        if (lane >= o) {
+            incl += up;
+            incl_some += up_some;
+        }
     }
-    if (lane == 31) sh.part[warp] = incl;
+    if (lane == 31) {
+        sh.slots[warp] = incl;
+        sh.some[warp] = incl_some;
+    }
     __syncthreads();
     long long before = incl - mine, total = 0;
+    int before_some = incl_some - some, total_some = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) before += sh.part[w];
-        total += sh.part[w];
+        if (w < warp) {
+            before += sh.slots[w];
+            before_some += sh.some[w];
+        }
+        total += sh.slots[w];
+        total_some += sh.some[w];
     }
     Split s;
-    s.units = total * heads;
-    s.G = (int)min((long long)gridDim.x, s.units);
+    s.extra = total * heads > ctas ? 1 : 0;
+    before += s.extra * before_some;
+    mine += s.extra * some;
+    s.units = (total + s.extra * total_some) * heads;
+    s.G = (int)min((long long)ctas, s.units);
     s.u = s.u1 = 0;
     if ((int)blockIdx.x < s.G) {
         s.u = Split::start(s.units, blockIdx.x, s.G);
@@ -137,7 +176,7 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
         if (x >= before && x < before + mine) {
             int64_t b = b0;
             for (;; ++b) {
-                const int n = (c.length(b) + kUnit - 1) / kUnit;
+                const int n = s.chunks_of<kUnit>(c.length(b));
                 if (x < before + n) break;
                 before += n;
             }
@@ -146,9 +185,10 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
         }
         __syncthreads();
         s.b = sh.b;
+        s.before = sh.before;
         s.len = c.length(s.b);
-        s.chunks = (s.len + kUnit - 1) / kUnit;
-        const long long r = s.u - sh.before * heads;
+        s.chunks = s.chunks_of<kUnit>(s.len);
+        const long long r = s.u - s.before * heads;
         s.h = (int)(r / s.chunks);
         s.chunk = (int)(r % s.chunks);
     }
@@ -162,8 +202,9 @@ __device__ __forceinline__ void split_next(Split& s, const Cache& c, int heads) 
     if (++s.h < heads) return;
     s.h = 0;
     do {
+        s.before += s.chunks;
         s.len = c.length(++s.b);
-        s.chunks = (s.len + kUnit - 1) / kUnit;
+        s.chunks = s.chunks_of<kUnit>(s.len);
     } while (s.chunks == 0);
 }
 

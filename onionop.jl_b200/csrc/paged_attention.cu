@@ -13,7 +13,7 @@
 // shared memory.  A (sequence, head tile) that lies in one CTA is written at once;
 // the others leave (maximum, sum, accumulator) in the workspace and a second launch
 // joins them.  The weights need the final lse, so the scores are kept (fp32,
-// workspace) and a third launch turns them into weights: 8 bytes per (query head,
+// workspace) and the second launch turns them into weights: 8 bytes per (query head,
 // slot) instead of reading K again (E·size).
 #include "paged.cuh"
 
@@ -82,7 +82,7 @@ attention_simt(AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, sub = lane & 3;
     const int heads = a.KH * a.tiles;
     let_next_start();
-    Split s = split_begin<kUnit>(a.c, a.B, heads, sh);
+    Split s = split_begin<kUnit>(a.c, a.B, heads, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (s.u < s.u1) {
@@ -106,8 +106,8 @@ attention_simt(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < COLS; ++i) acc[r][i] = 0.f;
         }
-        const int end = min(s.len, c1 * kUnit);
-        for (int key0 = c0 * kUnit + warp * kKeys; key0 < end; key0 += kUnit) {
+        const int end = s.end_slot<kUnit>(c1);
+        for (int key0 = s.first_slot<kUnit>(c0) + warp * kKeys; key0 < end; key0 += kUnit) {
             int64_t off[kKeys / 8];
             float sc[kKeys / 8][R];
 #pragma unroll
@@ -261,13 +261,13 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[W], const void* p, bool
     const int on = live;
     if constexpr (W == 4) {
         asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
-                     " @p ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];\n}"
+                     " @p ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n}"
                      : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]) : "l"(p), "r"(on));
     } else if constexpr (W == 2) {
-        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n @p ld.global.nc.v2.b32 {%0,%1}, [%2];\n}"
+        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n @p ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];\n}"
                      : "=&r"(r[0]), "=&r"(r[1]) : "l"(p), "r"(on));
     } else {
-        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.nc.b32 %0, [%1];\n}"
+        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.nc.L1::no_allocate.b32 %0, [%1];\n}"
                      : "=&r"(r[0]) : "l"(p), "r"(on));
     }
 }
@@ -298,26 +298,32 @@ template <int E> struct MmaShape {
     static constexpr int kUnit = 4 * kKeys;                         // slots per unit
 };
 
-// WT: head tiles (of 8) per CTA.  The warps of one key group share the K and V rows
-// they read (by L1), those of one head tile share the keys out.
-template <typename T, int E, int WT>
-__global__ void __launch_bounds__(kThreads, 3)
+// CTAs per SM.  What has to be in flight to keep HBM busy lies in registers, 8 KB a
+// warp, beside 32·NT for Oᵀ and 16·NT for Q: three CTAs of 168 registers a thread
+// (181 us for 64 sequences up to 8192) before two of 255 (194 us) or four that spill
+// (236 us); with two head tiles a warp, two.
+constexpr int mma_ctas(int NT) { return NT == 1 ? 3 : 2; }
+
+// NT: head tiles (of 8) per warp, which share the fragments of K and V.  WT: warps
+// that read the same keys for other head tiles; 4/WT warps share the keys out.
+template <typename T, int E, int NT, int WT, bool kWholeTiles>
+__global__ void __launch_bounds__(kThreads, mma_ctas(NT))
 attention_mma(AttnArgs a) {
     using S = MmaShape<E>;
-    constexpr int R = 8 * WT;
+    constexpr int R = 8 * NT * WT;
     constexpr int KW = E >= 32 ? 4 : 2, KC = E / (8 * KW);     // words per K load, loads per row
     constexpr int VW = E >= 64 ? 4 : E == 32 ? 2 : 1, VC = E / (16 * VW);
     constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
     __shared__ SplitShared sh;
-    __shared__ float wm[4][8], wl[4][8];
-    __shared__ __align__(16) float wacc[4][8][E];
+    __shared__ float wm[4][8 * NT], wl[4][8 * NT];
+    __shared__ __align__(16) float wacc[4][8 * NT][E];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, sub = lane & 3;
-    const int tile = warp % WT, part = warp / WT;
+    const int tile0 = warp % WT * NT, part = warp / WT;
     const int heads = a.KH * a.tiles;
     const T* K = static_cast<const T*>(a.k);
     const T* V = static_cast<const T*>(a.v);
     let_next_start();
-    Split s = split_begin<S::kUnit>(a.c, a.B, heads, sh);
+    Split s = split_begin<S::kUnit>(a.c, a.B, heads, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (s.u < s.u1) {
@@ -328,133 +334,151 @@ attention_mma(AttnArgs a) {
         const int qh0 = kvh * a.group + r0;
         const int* tab = a.c.table + (int64_t)s.b * a.c.max_pages;
         const int64_t ho = (int64_t)kvh * a.c.head_stride;
-        // Q: B fragments of all k16 steps; head gid of this warp's tile
-        uint32_t q[KC][KW];
-        {
-            const int r = tile * 8 + gid;
+        // Q: B fragments of all k16 steps; head gid of each of this warp's tiles
+        uint32_t q[NT][KC][KW];
+        float m[NT][2], l[NT][2], acc[NT][VC][VW][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = (tile0 + n) * 8 + gid;
             const T* row = static_cast<const T*>(a.q) + ((int64_t)s.b * a.QH + qh0 + r) * E;
 #pragma unroll
-            for (int c = 0; c < KC; ++c) load_words<KW>(q[c], row + (c * 4 + sub) * (2 * KW), r < rows);
+            for (int c = 0; c < KC; ++c) load_words<KW>(q[n][c], row + (c * 4 + sub) * (2 * KW), r < rows);
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int j = 0; j < VW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][c][j][i] = 0.f;
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float acc[VC][VW][4];
-#pragma unroll
-        for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int j = 0; j < VW; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[c][j][i] = 0.f;
-        const int end = min(s.len, c1 * S::kUnit);
+        const int end = s.end_slot<S::kUnit>(c1);
         constexpr int kStep = S::kKeys * (4 / WT);
-        constexpr int NO = S::kKeys > 32 ? 2 : 1;
+        // Where a step's rows are.  kWholeTiles (pages of a multiple of 16 slots): a tile of
+        // 16 keys lies in one page, one lookup per tile, the same for all lanes.  Else one
+        // per key, key i in lane i mod 32, handed out by shuffles.
+        constexpr int NO = kWholeTiles ? S::kTiles : S::kKeys > 32 ? 2 : 1;
         uint32_t kr[S::kTiles][2][KC][KW], vr[S::kTiles][4][VC][VW];
         int64_t off[NO], next[NO];
-        // offsets of a step's keys: key i in lane i mod 32
         auto find = [&](int64_t (&o)[NO], int key0) {
 #pragma unroll
             for (int i = 0; i < NO; ++i) {
-                const int key = key0 + i * 32 + (S::kKeys < 32 ? (lane & 15) : lane);
+                const int key = key0 + (kWholeTiles ? i * 16 : i * 32 + (S::kKeys < 32 ? (lane & 15) : lane));
                 o[i] = key < end ? a.c.offset(tab, key, ho) : -1;
             }
         };
-        auto load_k = [&](const int64_t (&o)[NO]) {
+        // Offset of key `at` + `mine` of the step that begins at key0 (at: the same for all lanes); negative: no row.
+        auto row_of = [&](const int64_t (&o)[NO], int key0, int at, int mine) -> int64_t {
+            if constexpr (kWholeTiles) {
+                const int64_t x = o[at / 16] + (at % 16 + mine) * a.c.row_stride;
+                return o[at / 16] >= 0 && key0 + at + mine < end ? x : -1;
+            } else {
+                return __shfl_sync(0xffffffffu, o[at / 32], at % 32 + mine);
+            }
+        };
+        auto load_k = [&](const int64_t (&o)[NO], int key0) {
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int at = t * 16 + i * 8;
-                    const int64_t x = __shfl_sync(0xffffffffu, o[at / 32], at % 32 + gid);
+                    const int64_t x = row_of(o, key0, t * 16 + i * 8, gid);
 #pragma unroll
                     for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], K + x + (c * 4 + sub) * (2 * KW), x >= 0);
                 }
         };
-        auto load_v = [&](const int64_t (&o)[NO]) {
+        auto load_v = [&](const int64_t (&o)[NO], int key0) {
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int at = t * 16 + (i >> 1) * 8 + (i & 1);
-                    const int64_t x = __shfl_sync(0xffffffffu, o[at / 32], at % 32 + 2 * sub);
+                    const int64_t x = row_of(o, key0, t * 16 + (i >> 1) * 8 + (i & 1), 2 * sub);
 #pragma unroll
                     for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], V + x + (c * 8 + gid) * (2 * VW), x >= 0);
                 }
         };
-        int key0 = c0 * S::kUnit + part * S::kKeys;
+        int key0 = s.first_slot<S::kUnit>(c0) + part * S::kKeys;
         if (key0 < end) {
             find(off, key0);
-            load_k(off);
-            load_v(off);
+            load_k(off, key0);
+            load_v(off, key0);
             find(next, key0 + kStep);
         }
         for (; key0 < end; key0 += kStep) {
-            float d[S::kTiles][4];
+            float d[NT][S::kTiles][4];
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
+                for (int t = 0; t < S::kTiles; ++t) {
 #pragma unroll
-                for (int c = 0; c < KC; ++c)
+                    for (int i = 0; i < 4; ++i) d[n][t][i] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < KW; w += 2)
-                        mma16816<T>(d[t], kr[t][0][c][w], kr[t][1][c][w], kr[t][0][c][w + 1], kr[t][1][c][w + 1], q[c][w],
-                                    q[c][w + 1]);
-            }
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int w = 0; w < KW; w += 2)
+                            mma16816<T>(d[n][t], kr[t][0][c][w], kr[t][1][c][w], kr[t][0][c][w + 1], kr[t][1][c][w + 1],
+                                        q[n][c][w], q[n][c][w + 1]);
+                }
             const bool more = key0 + kStep < end;
-            if (more) load_k(next);
+            if (more) load_k(next, key0 + kStep);
             // scores to weights against the running maximum; heads 2·sub and 2·sub + 1
-            float mx[2] = {m[0], m[1]};
+            uint32_t b[NT][S::kTiles][2][2];      // Pᵀ: [16-bit term][key half]
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float mx[2] = {m[n][0], m[n][1]};
+#pragma unroll
+                for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = t * 16 + i * 8;
+                        const bool live = row_of(off, key0, at, gid) >= 0;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float& x = d[n][t][i * 2 + j];
+                            x = live ? x * a.scale2 : -INFINITY;
+                            mx[j] = fmaxf(mx[j], x);
+                            const int key = key0 + at + gid, r = (tile0 + n) * 8 + 2 * sub + j;
+                            if (a.scores != nullptr && key < end && r < rows)
+                                a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = x;
+                        }
+                    }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+                }
+                float base[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) base[j] = mx[j] == -INFINITY ? 0.f : mx[j] - kShift;    // -Inf: no score yet
+                if (__any_sync(0xffffffffu, mx[0] != m[n][0] || mx[1] != m[n][1])) {
+                    const float f0 = fast_exp2(m[n][0] - kShift - base[0]), f1 = fast_exp2(m[n][1] - kShift - base[1]);
+                    l[n][0] *= f0;
+                    l[n][1] *= f1;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int j = 0; j < VW; ++j) {
+                            acc[n][c][j][0] *= f0;
+                            acc[n][c][j][1] *= f1;
+                            acc[n][c][j][2] *= f0;
+                            acc[n][c][j][3] *= f1;
+                        }
+                    m[n][0] = mx[0];
+                    m[n][1] = mx[1];
+                }
+#pragma unroll
+                for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float p0 = fast_exp2(d[n][t][i * 2] - base[0]), p1 = fast_exp2(d[n][t][i * 2 + 1] - base[1]);
+                        l[n][0] += p0;
+                        l[n][1] += p1;
+                        float e0, e1, u0, u1;
+                        b[n][t][0][i] = transpose8x8(pack2<T>(p0, p1, e0, e1));
+                        b[n][t][1][i] = transpose8x8(pack2<T>(e0, e1, u0, u1));
+                    }
+            }
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int at = t * 16 + i * 8;
-                    const bool live = __shfl_sync(0xffffffffu, off[at / 32], at % 32 + gid) >= 0;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float& x = d[t][i * 2 + j];
-                        x = live ? x * a.scale2 : -INFINITY;
-                        mx[j] = fmaxf(mx[j], x);
-                        const int key = key0 + at + gid, r = tile * 8 + 2 * sub + j;
-                        if (a.scores != nullptr && key < end && r < rows)
-                            a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = x;
-                    }
-                }
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
-            }
-            float base[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) base[j] = mx[j] == -INFINITY ? 0.f : mx[j] - kShift;    // -Inf: no score yet
-            if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
-                const float f0 = fast_exp2(m[0] - kShift - base[0]), f1 = fast_exp2(m[1] - kShift - base[1]);
-                l[0] *= f0;
-                l[1] *= f1;
-#pragma unroll
-                for (int c = 0; c < VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < VW; ++j) {
-                        acc[c][j][0] *= f0;
-                        acc[c][j][1] *= f1;
-                        acc[c][j][2] *= f0;
-                        acc[c][j][3] *= f1;
-                    }
-                m[0] = mx[0];
-                m[1] = mx[1];
-            }
-#pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) {
-                uint32_t b[2][2];      // [16-bit term][key half]
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float p0 = fast_exp2(d[t][i * 2] - base[0]), p1 = fast_exp2(d[t][i * 2 + 1] - base[1]);
-                    l[0] += p0;
-                    l[1] += p1;
-                    float e0, e1, u0, u1;
-                    b[0][i] = transpose8x8(pack2<T>(p0, p1, e0, e1));
-                    b[1][i] = transpose8x8(pack2<T>(e0, e1, u0, u1));
-                }
 #pragma unroll
                 for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -463,36 +487,38 @@ attention_mma(AttnArgs a) {
                         const uint32_t a1 = __byte_perm(vr[t][0][c][j], vr[t][1][c][j], 0x7632);
                         const uint32_t a2 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x5410);
                         const uint32_t a3 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x7632);
-                        mma16816<T>(acc[c][j], a0, a1, a2, a3, b[0][0], b[0][1]);
-                        mma16816<T>(acc[c][j], a0, a1, a2, a3, b[1][0], b[1][1]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][0][0], b[n][t][0][1]);
+                            mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][1][0], b[n][t][1][1]);
+                        }
                     }
-            }
-            if (more) load_v(next);
+            if (more) load_v(next, key0 + kStep);
 #pragma unroll
             for (int i = 0; i < NO; ++i) off[i] = next[i];
             find(next, key0 + 2 * kStep);
         }
         // join the warps of each head tile
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-            l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
-        }
-        if (gid == 0) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                wm[warp][2 * sub + j] = m[j] - kShift;
-                wl[warp][2 * sub + j] = l[j];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], o);
+                if (gid == 0) {
+                    wm[warp][n * 8 + 2 * sub + j] = m[n][j] - kShift;
+                    wl[warp][n * 8 + 2 * sub + j] = l[n][j];
+                }
             }
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int j = 0; j < VW; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        *reinterpret_cast<float2*>(&wacc[warp][n * 8 + 2 * sub + h][(c * 8 + gid) * (2 * VW) + 2 * j]) =
+                            make_float2(acc[n][c][j][h], acc[n][c][j][2 + h]);
         }
-#pragma unroll
-        for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int j = 0; j < VW; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    *reinterpret_cast<float2*>(&wacc[warp][2 * sub + h][(c * 8 + gid) * (2 * VW) + 2 * j]) =
-                        make_float2(acc[c][j][h], acc[c][j][2 + h]);
         __syncthreads();
         const bool whole = c0 == 0 && c1 == s.chunks;
         const int slot = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
@@ -501,7 +527,7 @@ attention_mma(AttnArgs a) {
             float mw[4 / WT], mx = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4 / WT; ++w) {
-                mw[w] = wm[w * WT + r / 8][r % 8];
+                mw[w] = wm[w * WT + r / (8 * NT)][r % (8 * NT)];
                 mx = fmaxf(mx, mw[w]);
             }
             const float base = mx == -INFINITY ? 0.f : mx;
@@ -509,8 +535,8 @@ attention_mma(AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < 4 / WT; ++w) {
                 const float f = fast_exp2(mw[w] - base);
-                sum = fmaf(wl[w * WT + r / 8][r % 8], f, sum);
-                ac = fmaf(wacc[w * WT + r / 8][r % 8][e], f, ac);
+                sum = fmaf(wl[w * WT + r / (8 * NT)][r % (8 * NT)], f, sum);
+                ac = fmaf(wacc[w * WT + r / (8 * NT)][r % (8 * NT)][e], f, ac);
             }
             if (whole) {
                 write_row<T, E>(a, s.b, qh0 + r, e, ac, mx, sum);
@@ -529,52 +555,117 @@ attention_mma(AttnArgs a) {
     }
 }
 
-// Joins the parts of the (sequence, head tile) whose first part CTA blockIdx.x wrote;
-// blockIdx.y is the row.  Part i lies in slot 2(c + i), the first in 2c + 1.
-template <typename T, int E, int R>
-__global__ void __launch_bounds__(E) attention_join(AttnArgs a) {
-    wait_before();
-    let_next_start();
-    const int c = blockIdx.x, r = blockIdx.y, e = threadIdx.x;
-    const int4 w = a.join[c];
-    const int r0 = (w.y % a.tiles) * R;
-    if (w.z == 0 || r0 + r >= a.group) return;
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int i = 0; i < w.z; ++i) {
-        const int slot = 2 * (c + i) + (i == 0 ? 1 : 0);
-        const float2 ml = a.part_ml[slot * R + r];
-        const float x = a.part_acc[((int64_t)slot * R + r) * E + e];
-        const float mx = fmaxf(m, ml.x);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        const float f0 = fast_exp2(m - base), f1 = fast_exp2(ml.x - base);
-        acc = acc * f0 + x * f1;
-        l = l * f0 + ml.y * f1;
+// What the parts of one row come to: maximum (log2 domain) and sum.  A warp; part i lies
+// in slot 2(c + i), the first in 2c + 1.
+__device__ __forceinline__ float2 join_ml(const float2* part_ml, int R, int c, int parts, int r) {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+        const float2 ml = part_ml[(2 * (c + i) + (i == 0 ? 1 : 0)) * R + r];
+        const float mx = fmaxf(m, ml.x), base = mx == -INFINITY ? 0.f : mx;
+        l = l * fast_exp2(m - base) + ml.y * fast_exp2(ml.x - base);
         m = mx;
     }
-    write_row<T, E>(a, w.x, (w.y / a.tiles) * a.group + r0 + r, e, acc, m, l);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+        const float mx = fmaxf(m, m2), base = mx == -INFINITY ? 0.f : mx;
+        l = l * fast_exp2(m - base) + l2 * fast_exp2(m2 - base);
+        m = mx;
+    }
+    return make_float2(m, l);
 }
 
-// weights[b][kv head][j] += Σ over the group of exp(s_j − lse).
-__global__ void __launch_bounds__(kThreads) attention_weights(AttnArgs a) {
-    __shared__ SplitShared sh;
+constexpr int kJoinThreads = 128;
+
+// Second launch.  blockIdx.y < rows: row blockIdx.y of the (sequence, head tile) whose
+// first part CTA blockIdx.x wrote, a quarter of the parts per warp.  blockIdx.y ==
+// rows (with weights): weights[b][kv head][j] += Σ over the group of exp(s_j − lse) for
+// a share of the slots; a split row's lse comes from its parts again, so that both run
+// at once.
+template <typename T, int E, int R, int kUnit>
+__global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int rows, int ctas) {
+    constexpr int LE = E / 4;                             // lanes per row of 16-byte vectors
+    constexpr int NP = kJoinThreads / LE;                 // parts at once
+    __shared__ __align__(16) union {
+        float acc[NP][E];
+        struct {
+            SplitShared split;
+            float lse2[32];
+        } w;
+    } sh;
+    static_assert(kThreads == kJoinThreads, "split_begin counts on kThreads threads");
     wait_before();
-    Split s = split_begin<kUnit>(a.c, a.B, a.KH, sh);
+    const int t = threadIdx.x;
+    if ((int)blockIdx.y < rows) {
+        const int c = blockIdx.x, r = blockIdx.y;
+        const int4 w = a.join[c];
+        const int r0 = (w.y % a.tiles) * R;
+        if (w.z == 0 || r0 + r >= a.group) return;
+        const float2 ml = join_ml(a.part_ml, R, c, w.z, r);
+        const float base = ml.x == -INFINITY ? 0.f : ml.x;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = t / LE; i < w.z; i += NP) {
+            const int slot = 2 * (c + i) + (i == 0 ? 1 : 0);
+            const float f = fast_exp2(a.part_ml[slot * R + r].x - base);
+            const float4 y = *reinterpret_cast<const float4*>(a.part_acc + ((int64_t)slot * R + r) * E + (t % LE) * 4);
+            x.x = fmaf(f, y.x, x.x);
+            x.y = fmaf(f, y.y, x.y);
+            x.z = fmaf(f, y.z, x.z);
+            x.w = fmaf(f, y.w, x.w);
+        }
+        *reinterpret_cast<float4*>(&sh.acc[t / LE][(t % LE) * 4]) = x;
+        __syncthreads();
+        if (t < E) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) sum += sh.acc[i][t];
+            write_row<T, E>(a, w.x, (w.y / a.tiles) * a.group + r0 + r, t, sum, ml.x, ml.y);
+        }
+        return;
+    }
+    // The first launch's split again.  Head tile h of sequence b has units
+    // [before·heads + h·chunks, ... + chunks), so which CTAs had them is known.
+    Split s = split_begin<kUnit>(a.c, a.B, a.KH * a.tiles, ctas, sh.w.split);
+    const long long units = s.units;
+    const int G = s.G;
     while (s.u < s.u1) {
         const int c0 = s.chunk;
         const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
-        const int end = min(s.len, c1 * kUnit);
-        const int64_t row0 = (int64_t)s.b * a.QH + s.h * a.group;
-        float* w = a.weights + ((int64_t)s.b * a.KH + s.h) * a.c.slots;
-        for (int j = c0 * kUnit + threadIdx.x; j < end; j += kThreads) {
-            float sum = 0.f;
-            for (int g = 0; g < a.group; ++g) {
-                const float lse2 = a.lse[row0 + g] * kLog2e;
-                sum += lse2 == -INFINITY ? 0.f : fast_exp2(a.scores[(row0 + g) * a.c.slots + j] - lse2);
+        const int end = s.end_slot<kUnit>(c1);
+        const int kvh = s.h / a.tiles;
+        // a chunk's weights are added up by the CTA that has it for the first head tile
+        if (s.h % a.tiles == 0) {
+            const int64_t row0 = (int64_t)s.b * a.QH + kvh * a.group;
+            float* w = a.weights + ((int64_t)s.b * a.KH + kvh) * a.c.slots;
+            for (int g0 = 0; g0 < a.group; g0 += 32) {
+                __syncthreads();
+                for (int g = t / 32; g < min(32, a.group - g0); g += kJoinThreads / 32) {
+                    const int tile = (g0 + g) / R, r = (g0 + g) % R;
+                    const long long u = (s.before * a.KH * a.tiles) + (long long)(s.h + tile) * s.chunks;
+                    const int first = Split::owner(units, u, G), last = Split::owner(units, u + s.chunks - 1, G);
+                    float lse2;
+                    if (first == last) {
+                        lse2 = a.lse[row0 + g0 + g] * kLog2e;
+                    } else {
+                        const float2 ml = join_ml(a.part_ml, R, first, last - first + 1, r);
+                        lse2 = ml.y > 0.f || ml.y != ml.y ? ml.x + log2f(ml.y) : -INFINITY;
+                    }
+                    if (t % 32 == 0) sh.w.lse2[g] = lse2;
+                }
+                __syncthreads();
+                for (int j = s.first_slot<kUnit>(c0) + t; j < end; j += kJoinThreads) {
+                    float sum = 0.f;
+                    for (int g = 0; g < min(32, a.group - g0); ++g)
+                        sum += sh.w.lse2[g] == -INFINITY
+                                   ? 0.f : fast_exp2(a.scores[(row0 + g0 + g) * a.c.slots + j] - sh.w.lse2[g]);
+                    w[j] += sum;
+                }
             }
-            w[j] += sum;
         }
         s.u += c1 - c0;
-        if (s.u < s.u1) split_next<kUnit>(s, a.c, a.KH);
+        if (s.u < s.u1) split_next<kUnit>(s, a.c, a.KH * a.tiles);
     }
 }
 
@@ -612,18 +703,22 @@ int check_heads(int64_t E, int64_t QH, int64_t KH, int64_t B) {
 template <typename T, int E, int R>
 int launch(const AttnArgs& a, cudaStream_t s) {
     int G;
-    if constexpr (std::is_same<T, float>::value) {
+    constexpr bool f32 = std::is_same<T, float>::value;
+    if constexpr (f32) {
         G = std::min(kMaxCtas, 4 * num_sms());
         attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
     } else {
-        G = std::min(kMaxCtas, 3 * num_sms());
-        attention_mma<T, E, R / 8><<<G, kThreads, 0, s>>>(a);
+        constexpr int NT = R == 8 ? 1 : 2, WT = R / (8 * NT);
+        G = std::min(kMaxCtas, mma_ctas(NT) * num_sms());
+        if (a.c.page_size.d % 16 == 0)
+            attention_mma<T, E, NT, WT, true><<<G, kThreads, 0, s>>>(a);
+        else
+            attention_mma<T, E, NT, WT, false><<<G, kThreads, 0, s>>>(a);
     }
     if (const int rc = check_launch("paged_attention")) return rc;
-    if (const int rc = launch_dependent("paged_attention", attention_join<T, E, R>, dim3(G, R), dim3(E), 0, s, a))
-        return rc;
-    if (a.weights == nullptr) return NNOP_OK;
-    return launch_dependent("paged_attention", attention_weights, dim3(G), dim3(kThreads), 0, s, a);
+    const int rows = std::min(R, a.group);
+    return launch_dependent("paged_attention", attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit>,
+                            dim3(G, rows + (a.weights != nullptr ? 1 : 0)), dim3(kJoinThreads), 0, s, a, rows, G);
 }
 
 template <typename T, int E>
