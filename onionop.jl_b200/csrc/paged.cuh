@@ -119,10 +119,11 @@ struct Split {
     __device__ __forceinline__ int end_slot(int c1) const { return min(len, (c1 - extra) * kUnit); }
 };
 
-// Block-wide (kThreads threads): this CTA's share, set to its first unit.  The units
-// are counted as `heads` head tiles and `ctas` CTAs make them.
+// Block-wide (kThreads threads): the units as `ctas` CTAs share them (extra, G), and
+// part `index` of `parts` of them, set to its first unit.
 template <int kUnit>
-__device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, int ctas, SplitShared& sh) {
+__device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, int ctas, int index, int parts,
+                                             SplitShared& sh) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t per = (B + kThreads - 1) / kThreads;
     const int64_t b0 = min((int64_t)t * per, B), b1 = min(b0 + per, B);
@@ -167,9 +168,10 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
     s.units = (total + s.extra * total_some) * heads;
     s.G = (int)min((long long)ctas, s.units);
     s.u = s.u1 = 0;
-    if ((int)blockIdx.x < s.G) {
-        s.u = Split::start(s.units, blockIdx.x, s.G);
-        s.u1 = Split::start(s.units, blockIdx.x + 1, s.G);
+    parts = (int)min((long long)parts, s.units);
+    if (index < parts) {
+        s.u = Split::start(s.units, index, parts);
+        s.u1 = Split::start(s.units, index + 1, parts);
     }
     if (s.u < s.u1) {
         const long long x = s.u / heads;      // in sequence b: before(b) <= x < before(b) + chunks(b)

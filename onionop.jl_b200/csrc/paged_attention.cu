@@ -82,7 +82,7 @@ attention_simt(AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, sub = lane & 3;
     const int heads = a.KH * a.tiles;
     let_next_start();
-    Split s = split_begin<kUnit>(a.c, a.B, heads, gridDim.x, sh);
+    Split s = split_begin<kUnit>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (s.u < s.u1) {
@@ -323,7 +323,7 @@ attention_mma(AttnArgs a) {
     const T* K = static_cast<const T*>(a.k);
     const T* V = static_cast<const T*>(a.v);
     let_next_start();
-    Split s = split_begin<S::kUnit>(a.c, a.B, heads, gridDim.x, sh);
+    Split s = split_begin<S::kUnit>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (s.u < s.u1) {
@@ -353,55 +353,56 @@ attention_mma(AttnArgs a) {
                     for (int i = 0; i < 4; ++i) acc[n][c][j][i] = 0.f;
         }
         const int end = s.end_slot<S::kUnit>(c1);
-        constexpr int kStep = S::kKeys * (4 / WT);
-        // Where a step's rows are.  kWholeTiles (pages of a multiple of 16 slots): a tile of
-        // 16 keys lies in one page, one lookup per tile, the same for all lanes.  Else one
-        // per key, key i in lane i mod 32, handed out by shuffles.
-        constexpr int NO = kWholeTiles ? S::kTiles : S::kKeys > 32 ? 2 : 1;
         uint32_t kr[S::kTiles][2][KC][KW], vr[S::kTiles][4][VC][VW];
-        int64_t off[NO], next[NO];
-        auto find = [&](int64_t (&o)[NO], int key0) {
-#pragma unroll
-            for (int i = 0; i < NO; ++i) {
-                const int key = key0 + (kWholeTiles ? i * 16 : i * 32 + (S::kKeys < 32 ? (lane & 15) : lane));
-                o[i] = key < end ? a.c.offset(tab, key, ho) : -1;
-            }
-        };
-        // Offset of key `at` + `mine` of the step that begins at key0 (at: the same for all lanes); negative: no row.
-        auto row_of = [&](const int64_t (&o)[NO], int key0, int at, int mine) -> int64_t {
+        uint32_t live = 0;             // bit 2t + i: this lane's key 16t + 8i + gid has a row
+        // Where a step's rows are (negative offset: no row).  kWholeTiles (pages of a multiple
+        // of 16 slots): a tile of 16 keys lies in one page, one lookup for all lanes, made a
+        // step ahead (168 us for 64 sequences up to 8192; 175 when it is made with the loads).
+        // Else one lookup for each row a lane reads (pages of 20: 191 us; a step ahead in
+        // other lanes and handed out by shuffles: 221).
+        int64_t tiles[S::kTiles];
+        auto find = [&](int key0) {
             if constexpr (kWholeTiles) {
-                const int64_t x = o[at / 16] + (at % 16 + mine) * a.c.row_stride;
-                return o[at / 16] >= 0 && key0 + at + mine < end ? x : -1;
-            } else {
-                return __shfl_sync(0xffffffffu, o[at / 32], at % 32 + mine);
+#pragma unroll
+                for (int t = 0; t < S::kTiles; ++t)
+                    tiles[t] = key0 + t * 16 < end ? a.c.offset(tab, key0 + t * 16, ho) : -1;
             }
         };
-        auto load_k = [&](const int64_t (&o)[NO], int key0) {
+        auto row_at = [&](int t, int key, int mine) -> int64_t {
+            if (key + mine >= end) return -1;
+            if constexpr (kWholeTiles) return tiles[t] < 0 ? -1 : tiles[t] + mine * a.c.row_stride;
+            return a.c.offset(tab, key + mine, ho);
+        };
+        auto load_k = [&](int key0) {
+            uint32_t has = 0;
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int64_t x = row_of(o, key0, t * 16 + i * 8, gid);
+                    const int64_t x = row_at(t, key0 + t * 16, i * 8 + gid);
+                    has |= (uint32_t)(x >= 0) << (2 * t + i);
 #pragma unroll
                     for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], K + x + (c * 4 + sub) * (2 * KW), x >= 0);
                 }
+            return has;
         };
-        auto load_v = [&](const int64_t (&o)[NO], int key0) {
+        auto load_v = [&](int key0) {
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int64_t x = row_of(o, key0, t * 16 + (i >> 1) * 8 + (i & 1), 2 * sub);
+                    const int64_t x = row_at(t, key0 + t * 16, (i >> 1) * 8 + (i & 1) + 2 * sub);
 #pragma unroll
                     for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], V + x + (c * 8 + gid) * (2 * VW), x >= 0);
                 }
         };
+        constexpr int kStep = S::kKeys * (4 / WT);
         int key0 = s.first_slot<S::kUnit>(c0) + part * S::kKeys;
         if (key0 < end) {
-            find(off, key0);
-            load_k(off, key0);
-            load_v(off, key0);
-            find(next, key0 + kStep);
+            find(key0);
+            live = load_k(key0);
+            load_v(key0);
+            find(key0 + kStep);
         }
         for (; key0 < end; key0 += kStep) {
             float d[NT][S::kTiles][4];
@@ -419,7 +420,7 @@ attention_mma(AttnArgs a) {
                                         q[n][c][w], q[n][c][w + 1]);
                 }
             const bool more = key0 + kStep < end;
-            if (more) load_k(next, key0 + kStep);
+            const uint32_t next = more ? load_k(key0 + kStep) : 0;
             // scores to weights against the running maximum; heads 2·sub and 2·sub + 1
             uint32_t b[NT][S::kTiles][2][2];      // Pᵀ: [16-bit term][key half]
 #pragma unroll
@@ -430,11 +431,11 @@ attention_mma(AttnArgs a) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int at = t * 16 + i * 8;
-                        const bool live = row_of(off, key0, at, gid) >= 0;
+                        const bool on = live >> (2 * t + i) & 1;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             float& x = d[n][t][i * 2 + j];
-                            x = live ? x * a.scale2 : -INFINITY;
+                            x = on ? x * a.scale2 : -INFINITY;
                             mx[j] = fmaxf(mx[j], x);
                             const int key = key0 + at + gid, r = (tile0 + n) * 8 + 2 * sub + j;
                             if (a.scores != nullptr && key < end && r < rows)
@@ -493,10 +494,9 @@ attention_mma(AttnArgs a) {
                             mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][1][0], b[n][t][1][1]);
                         }
                     }
-            if (more) load_v(next, key0 + kStep);
-#pragma unroll
-            for (int i = 0; i < NO; ++i) off[i] = next[i];
-            find(next, key0 + 2 * kStep);
+            if (more) load_v(key0 + kStep);
+            live = next;
+            find(key0 + 2 * kStep);
         }
         // join the warps of each head tile
 #pragma unroll
@@ -578,11 +578,10 @@ __device__ __forceinline__ float2 join_ml(const float2* part_ml, int R, int c, i
 
 constexpr int kJoinThreads = 128;
 
-// Second launch.  blockIdx.y < rows: row blockIdx.y of the (sequence, head tile) whose
-// first part CTA blockIdx.x wrote, a quarter of the parts per warp.  blockIdx.y ==
-// rows (with weights): weights[b][kv head][j] += Σ over the group of exp(s_j − lse) for
-// a share of the slots; a split row's lse comes from its parts again, so that both run
-// at once.
+// Second launch.  Blocks below rows·ctas: row blockIdx.x mod rows of the (sequence,
+// head tile) whose first part CTA blockIdx.x / rows wrote.  The others (with weights):
+// weights[b][kv head][j] += Σ over the group of exp(s_j − lse) for a share of the
+// slots; a split row's lse comes from its parts again, so that both run at once.
 template <typename T, int E, int R, int kUnit>
 __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int rows, int ctas) {
     constexpr int LE = E / 4;                             // lanes per row of 16-byte vectors
@@ -597,8 +596,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int r
     static_assert(kThreads == kJoinThreads, "split_begin counts on kThreads threads");
     wait_before();
     const int t = threadIdx.x;
-    if ((int)blockIdx.y < rows) {
-        const int c = blockIdx.x, r = blockIdx.y;
+    if ((int)blockIdx.x < rows * ctas) {
+        const int c = blockIdx.x / rows, r = blockIdx.x % rows;
         const int4 w = a.join[c];
         const int r0 = (w.y % a.tiles) * R;
         if (w.z == 0 || r0 + r >= a.group) return;
@@ -627,7 +626,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int r
     }
     // The first launch's split again.  Head tile h of sequence b has units
     // [before·heads + h·chunks, ... + chunks), so which CTAs had them is known.
-    Split s = split_begin<kUnit>(a.c, a.B, a.KH * a.tiles, ctas, sh.w.split);
+    Split s = split_begin<kUnit>(a.c, a.B, a.KH * a.tiles, ctas, blockIdx.x - rows * ctas, gridDim.x - rows * ctas, sh.w.split);
     const long long units = s.units;
     const int G = s.G;
     while (s.u < s.u1) {
@@ -655,12 +654,24 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int r
                     if (t % 32 == 0) sh.w.lse2[g] = lse2;
                 }
                 __syncthreads();
-                for (int j = s.first_slot<kUnit>(c0) + t; j < end; j += kJoinThreads) {
-                    float sum = 0.f;
-                    for (int g = 0; g < min(32, a.group - g0); ++g)
-                        sum += sh.w.lse2[g] == -INFINITY
-                                   ? 0.f : fast_exp2(a.scores[(row0 + g0 + g) * a.c.slots + j] - sh.w.lse2[g]);
-                    w[j] += sum;
+                // four slots a thread at once: their loads do not wait for one another
+                const int heads = min(32, a.group - g0);
+                for (int j0 = s.first_slot<kUnit>(c0) + t; j0 < end; j0 += 4 * kJoinThreads) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int g = 0; g < heads; ++g) {
+                        const float lse2 = sh.w.lse2[g];
+                        const float* sc = a.scores + (row0 + g0 + g) * a.c.slots;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = j0 + i * kJoinThreads;
+                            if (j < end && lse2 != -INFINITY) sum[i] += fast_exp2(sc[j] - lse2);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = j0 + i * kJoinThreads;
+                        if (j < end) w[j] += sum[i];
+                    }
                 }
             }
         }
@@ -718,7 +729,7 @@ int launch(const AttnArgs& a, cudaStream_t s) {
     if (const int rc = check_launch("paged_attention")) return rc;
     const int rows = std::min(R, a.group);
     return launch_dependent("paged_attention", attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit>,
-                            dim3(G, rows + (a.weights != nullptr ? 1 : 0)), dim3(kJoinThreads), 0, s, a, rows, G);
+                            dim3(G * rows + (a.weights != nullptr ? 8 * num_sms() : 0)), dim3(kJoinThreads), 0, s, a, rows, G);
 }
 
 template <typename T, int E>

@@ -10,6 +10,10 @@
 // slot for the choice and 4·E·size bytes per kept slot for the move.
 #include "paged.cuh"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 namespace nnop {
 namespace paged {
 
@@ -58,71 +62,95 @@ struct AppendArgs {
     void *q_out, *k_cache, *v_cache;
     int* new_lengths;
     Cache c;
-    int64_t T, B, cos_batch;
+    FastDiv T;
+    int64_t tokens, B, cos_batch;      // tokens = B·T
     int QH, KH;
 };
 
 constexpr int kAppendBlock = 256;
+constexpr int kAppendHeads = 4;      // heads per thread
 
-// A thread owns one 16-byte vector of the first half of a (head, token) row and its
-// partner E/2 further on: the pair that RoPE rotates.
+// A thread owns one 16-byte vector of the first half of a token's rows and its partner
+// E/2 further on (the pair that RoPE rotates) for kAppendHeads heads of q, of k or of v
+// (blockIdx.y): the angles, the page and the index arithmetic are fetched once for all
+// of them, and all rows are loaded before any is used.  Four prompts of 8192 tokens (32 +
+// 8 heads of 128, bf16, 772 MB): 117 us, 6.59 TB/s, with streaming stores; 175 us with
+// plain ones, 126 with two heads per thread, 117 with eight.
 template <typename T, int E>
 __global__ void __launch_bounds__(kAppendBlock) append_kernel(AppendArgs a) {
     constexpr int VEC = 16 / sizeof(T), HALF = E / 2, NH = HALF / VEC;
-    const int heads = a.QH + 2 * a.KH;      // rows of q, then k, then v
-    const int64_t total = a.B * heads * a.T * NH;
-    const int64_t first = (int64_t)blockIdx.x * kAppendBlock + threadIdx.x;
-    if (first < a.B) {
-        const int n = a.n_new ? min(max(a.n_new[first], 0), (int)a.T) : (int)a.T;
-        a.new_lengths[first] = (int)min((int64_t)a.c.length(first) + n, (int64_t)a.c.slots);
+    const int64_t i = (int64_t)blockIdx.x * kAppendBlock + threadIdx.x;
+    if (blockIdx.y == 0 && i < a.B) {
+        const int most = a.tokens > 0 ? (int)a.T.d : 0;
+        const int n = a.n_new ? min(max(a.n_new[i], 0), most) : most;
+        a.new_lengths[i] = (int)min((int64_t)a.c.length(i) + n, (int64_t)a.c.slots);
     }
-    for (int64_t i = first; i < total; i += (int64_t)gridDim.x * kAppendBlock) {
-        const int u = (int)(i % NH);
-        int64_t r = i / NH;
-        const int t = (int)(r % a.T);
-        r /= a.T;
-        const int h = (int)(r % heads);
-        const int64_t b = r / heads;
-        const bool is_q = h < a.QH, is_v = h >= a.QH + a.KH;
-        const T* src;
-        T* dst;
-        if (is_q) {
-            const int64_t off = ((b * a.QH + h) * a.T + t) * E;
-            src = static_cast<const T*>(a.q) + off;
-            dst = static_cast<T*>(a.q_out) + off;
-        } else {
-            const int n = a.n_new ? min(a.n_new[b], (int)a.T) : (int)a.T;
-            const int64_t slot = (int64_t)a.c.length(b) + t;
-            if (t >= n || slot >= a.c.slots) continue;
-            const int kvh = h - a.QH - (is_v ? a.KH : 0);
-            const int64_t to = a.c.offset(a.c.table + b * a.c.max_pages, (int)slot, (int64_t)kvh * a.c.head_stride);
-            if (to < 0) continue;
-            src = static_cast<const T*>(is_v ? a.v : a.k) + ((b * a.KH + kvh) * a.T + t) * E;
-            dst = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + to;
+    if (i >= a.tokens * NH) return;
+    const int u = (int)(i % NH);
+    const uint32_t r = (uint32_t)(i / NH);
+    const int64_t b = a.T.div(r);
+    const int t = (int)(r - (uint32_t)b * a.T.d);
+    const int gq = (a.QH + kAppendHeads - 1) / kAppendHeads, gk = (a.KH + kAppendHeads - 1) / kAppendHeads;
+    const int g = blockIdx.y;
+    const bool is_q = g < gq, is_v = g >= gq + gk;
+    const int h0 = (is_q ? g : is_v ? g - gq - gk : g - gq) * kAppendHeads;
+    const int H = is_q ? a.QH : a.KH;
+    const int64_t step = (int64_t)a.T.d * E;       // between heads of the new rows
+    const int64_t at = ((b * H + h0) * a.T.d + t) * E + u * VEC;
+    const T* src = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + at;
+    T* dst;
+    int64_t dst_step;
+    if (is_q) {
+        dst = static_cast<T*>(a.q_out) + at;
+        dst_step = step;
+    } else {
+        const int64_t slot = (int64_t)a.c.length(b) + t;
+        if ((a.n_new && t >= a.n_new[b]) || slot >= a.c.slots) return;
+        const int64_t to = a.c.offset(a.c.table + b * a.c.max_pages, (int)slot, (int64_t)h0 * a.c.head_stride);
+        if (to < 0) return;
+        dst = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + to + u * VEC;
+        dst_step = a.c.head_stride;
+    }
+    Vec<T, VEC> x[kAppendHeads], y[kAppendHeads];
+#pragma unroll
+    for (int j = 0; j < kAppendHeads; ++j)
+        if (h0 + j < H) {
+            x[j] = ldg_stream<T, VEC>(src + j * step);
+            y[j] = ldg_stream<T, VEC>(src + j * step + HALF);
         }
-        Vec<T, VEC> x = ldg_stream<T, VEC>(src + u * VEC), y = ldg_stream<T, VEC>(src + u * VEC + HALF);
-        if (!is_v && a.cos_t != nullptr) {
-            const int64_t at = ((a.cos_batch == 1 ? 0 : b) * a.T + t) * E + u * VEC;
+    if (!is_v && a.cos_t != nullptr) {
+        const int64_t ca = ((a.cos_batch == 1 ? 0 : b) * a.T.d + t) * E + u * VEC;
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            c[e] = __ldg(a.cos_t + ca + e);
+            s[e] = __ldg(a.sin_t + ca + e);
+        }
+#pragma unroll
+        for (int j = 0; j < kAppendHeads; ++j)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float c = __ldg(a.cos_t + at + e), s = __ldg(a.sin_t + at + e);
                 // the order of roundings that nnop_llama_rope's results have
-                const float x1 = to_f(x.v[e]), x2 = to_f(y.v[e]);
-                x.v[e] = from_f<T>(fmaf(x1, c, -__fmul_rn(x2, s)));
-                y.v[e] = from_f<T>(fmaf(x2, c, __fmul_rn(x1, s)));
+                const float x1 = to_f(x[j].v[e]), x2 = to_f(y[j].v[e]);
+                x[j].v[e] = from_f<T>(fmaf(x1, c[e], -__fmul_rn(x2, s[e])));
+                y[j].v[e] = from_f<T>(fmaf(x2, c[e], __fmul_rn(x1, s[e])));
             }
-        }
-        *reinterpret_cast<Vec<T, VEC>*>(dst + u * VEC) = x;
-        *reinterpret_cast<Vec<T, VEC>*>(dst + u * VEC + HALF) = y;
     }
+#pragma unroll
+    for (int j = 0; j < kAppendHeads; ++j)
+        if (h0 + j < H) {
+            st_stream<T, VEC>(dst + j * dst_step, x[j]);
+            st_stream<T, VEC>(dst + j * dst_step + HALF, y[j]);
+        }
 }
 
 template <typename T, int E>
 int launch_append(const AppendArgs& a, cudaStream_t s) {
     constexpr int NH = E / 2 / (16 / (int)sizeof(T));
-    const int64_t items = std::max(a.B * (a.QH + 2 * a.KH) * a.T * NH, a.B);
-    const int64_t grid = std::min((items + kAppendBlock - 1) / kAppendBlock, (int64_t)1 << 30);
-    append_kernel<T, E><<<(unsigned)grid, kAppendBlock, 0, s>>>(a);
+    const int64_t items = std::max(a.tokens * NH, a.B);
+    const unsigned grid = (unsigned)((items + kAppendBlock - 1) / kAppendBlock);
+    const unsigned groups = (a.QH + kAppendHeads - 1) / kAppendHeads + 2 * ((a.KH + kAppendHeads - 1) / kAppendHeads);
+    append_kernel<T, E><<<dim3(grid, groups), kAppendBlock, 0, s>>>(a);
     return check_launch("paged_append");
 }
 
@@ -150,117 +178,226 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kDigits = 3;                                   // of 11, 11 and 10 bits
+constexpr int kBins = 2048;
+constexpr size_t kHistBytes = sizeof(int) * kDigits * kBins;
+constexpr int kMostKeys = 48 * 1024;                         // of a CTA's share in shared memory
 
-// One CTA per (sequence, KV head): the (budget − recent)-th largest weight by four
-// counting passes over 8 bits each, then the kept slots in order.
-__global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a) {
-    __shared__ int hist[256];
-    __shared__ int pick[2];
-    __shared__ int warp_gt[32], warp_eq[32];
+__device__ __forceinline__ int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+
+// The slots to keep of one (sequence, KV head): a cluster of 1 to 8 CTAs, each with a
+// contiguous share of the slots and its keys in shared memory (read once; a share of
+// more than kMostKeys is read again).  The (budget − recent)-th largest key is found
+// digit by digit: every CTA counts its keys by the digit, sums the cluster's counts
+// through distributed shared memory and walks them from the top.  Then each CTA writes
+// its kept slots in order, behind those of the CTAs in front of it: a slot's place is
+// (larger keys in front) + min(equal keys in front, equals to keep).
+__global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a, int most_keys) {
+    extern __shared__ int smem[];
+    int* hist = smem;                                        // [kDigits][kBins]
+    uint32_t* keys = reinterpret_cast<uint32_t*>(smem + kDigits * kBins);
+    __shared__ int pick[2], warp_sum[kSelectWarps], warp_eq[kSelectWarps], mine[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t b = blockIdx.x / a.KH;
-    const float* w = a.weights + (int64_t)blockIdx.x * a.c.slots;
-    float* nw = a.new_weights + (int64_t)blockIdx.x * a.new_slots;
-    int* kept = a.kept + (int64_t)blockIdx.x * a.budget;
+    let_next_start();
+    const int64_t row = blockIdx.x / C;
+    const int64_t b = row / a.KH;
+    const float* w = a.weights + row * a.c.slots;
+    float* nw = a.new_weights + row * a.new_slots;
+    int* kept = a.kept + row * a.budget;
     const int n = a.c.length(b), count = min(n, a.budget);
-    if (blockIdx.x % a.KH == 0 && t == 0) a.new_lengths[b] = count;
-    for (int i = count + t; i < a.budget; i += kSelectThreads) kept[i] = -1;
-    for (int i = count + t; i < a.new_slots; i += kSelectThreads) nw[i] = 0.f;
+    const int gt0 = rank * kSelectThreads + t, all = C * kSelectThreads;
+    if (row % a.KH == 0 && gt0 == 0) a.new_lengths[b] = count;
+    for (int i = count + gt0; i < a.budget; i += all) kept[i] = -1;
+    for (int i = count + gt0; i < a.new_slots; i += all) nw[i] = 0.f;
     const int last = n <= a.budget ? n : min(a.recent, a.budget);   // slots kept unseen
     const int cand = n - last;
     const int need = count - last;                                  // of the first `cand`
-    for (int i = t; i < last; i += kSelectThreads) {
-        kept[need + i] = cand + i;
-        nw[need + i] = w[cand + i];
+    for (int i = gt0; i < last; i += all) kept[need + i] = cand + i;
+    if (need == 0) return;                                   // the same for the whole cluster
+    const int share = (cand + C - 1) / C;
+    const int i0 = min(rank * share, cand), size = min(share, cand - i0);
+    const bool held = size <= most_keys;
+    for (int i = t; i < kDigits * kBins; i += kSelectThreads) hist[i] = 0;
+    if (held) {
+#pragma unroll 4
+        for (int i = t; i < size; i += kSelectThreads) keys[i] = order_key(w[i0 + i]);
     }
-    if (need == 0) return;
-    uint32_t prefix = 0;
-    int rank = need;            // the wanted key is the rank-th largest of those with this prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int i = t; i < cand; i += kSelectThreads) {
-            const uint32_t key = order_key(w[i]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+    __syncthreads();
+    uint32_t prefix = 0;        // digits of the wanted key so far
+    int left = need;            // it is the left-th largest of the keys that begin so
+    for (int d = 0; d < kDigits; ++d) {
+        const int shift = digit_shift(d), above = d == 0 ? 0 : digit_shift(d - 1);
+        const int bins = d == 2 ? 1024 : 2048;
+        int* h = hist + d * kBins;
+        for (int i = t; i < size; i += kSelectThreads) {
+            const uint32_t key = held ? keys[i] : order_key(w[i0 + i]);
+            if (d == 0 || key >> above == prefix) atomicAdd(&h[(key >> shift) & (bins - 1)], 1);
         }
-        __syncthreads();
-        if (t == 0) {
-            int d = 255, r = rank;
-            while (hist[d] < r) r -= hist[d--];
-            pick[0] = d;
-            pick[1] = r;
-        }
-        __syncthreads();
-        prefix = prefix << 8 | (uint32_t)pick[0];
-        rank = pick[1];
-    }
-    // keys above `prefix` are kept, and the first `rank` that equal it
-    int gt = 0, eq = 0;         // in front of this tile
-    for (int i0 = 0; i0 < cand; i0 += kSelectThreads) {
-        const int i = i0 + t;
-        const float x = i < cand ? w[i] : 0.f;
-        const uint32_t key = order_key(x);
-        const bool is_gt = i < cand && key > prefix, is_eq = i < cand && key == prefix;
-        const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-        if (lane == 0) {
-            warp_gt[warp] = __popc(mg);
-            warp_eq[warp] = __popc(me);
-        }
-        __syncthreads();
-        int g = gt + __popc(mg & ((1u << lane) - 1)), e = eq + __popc(me & ((1u << lane) - 1));
-        for (int k = 0; k < 32; ++k) {
-            if (k < warp) {
-                g += warp_gt[k];
-                e += warp_eq[k];
+        cluster.sync();
+        // thread t has the t-th pair of bins from the top
+        const int top = bins - 1 - 2 * t;
+        int n1 = 0, n0 = 0;
+        if (top > 0) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c >= C) break;
+                const int2 x = *reinterpret_cast<const int2*>(cluster.map_shared_rank(h, c) + top - 1);
+                n0 += x.x;
+                n1 += x.y;
             }
-            gt += warp_gt[k];
-            eq += warp_eq[k];
         }
-        if (is_gt || (is_eq && e < rank)) {
-            const int at = g + min(e, rank);
-            kept[at] = i;
-            nw[at] = x;
+        int incl = n0 + n1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        int over = incl - n0 - n1;      // keys with a larger digit
+        over += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+        if (over < left && left <= over + n1) {
+            pick[0] = top;
+            pick[1] = left - over;
+        } else if (over + n1 < left && left <= over + n1 + n0) {
+            pick[0] = top - 1;
+            pick[1] = left - over - n1;
         }
         __syncthreads();
+        prefix = prefix << (d == 2 ? 10 : 11) | (uint32_t)pick[0];
+        left = pick[1];
     }
+    // Larger keys are kept, and the first `left` that equal it.  Each warp has a contiguous run.
+    const int run = ((size + kSelectWarps - 1) / kSelectWarps + 31) & ~31;
+    const int r0 = min(warp * run, size), r1 = min(r0 + run, size);
+    int gt = 0, eq = 0;
+    for (int i = r0 + lane; i < r1; i += 32) {
+        const uint32_t key = held ? keys[i] : order_key(w[i0 + i]);
+        gt += key > prefix;
+        eq += key == prefix;
+    }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    __syncthreads();
+    if (lane == 0) {
+        warp_sum[warp] = gt;
+        warp_eq[warp] = eq;
+    }
+    __syncthreads();
+    const int gt_all = __reduce_add_sync(0xffffffffu, warp_sum[lane]);
+    const int eq_all = __reduce_add_sync(0xffffffffu, warp_eq[lane]);
+    if (t == 0) {
+        mine[0] = gt_all;
+        mine[1] = eq_all;
+    }
+    cluster.sync();
+    gt = eq = 0;
+    for (int c = 0; c < rank; ++c) {
+        const int* other = cluster.map_shared_rank(mine, c);
+        gt += other[0];
+        eq += other[1];
+    }
+    gt += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+    eq += __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0);
+    for (int k0 = r0; k0 < r1; k0 += 32) {
+        const int i = k0 + lane;
+        const uint32_t key = i >= r1 ? 0 : held ? keys[i] : order_key(w[i0 + i]);
+        const bool is_gt = i < r1 && key > prefix, is_eq = i < r1 && key == prefix;
+        const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+        const uint32_t before = (1u << lane) - 1;
+        const int g = gt + __popc(mg & before), e = eq + __popc(me & before);
+        if (is_gt || (is_eq && e < left)) kept[g + min(e, left)] = i0 + i;
+        gt += __popc(mg);
+        eq += __popc(me);
+    }
+    cluster.sync();             // no CTA leaves while another may read its shared memory
 }
 
 constexpr int kMoveBlock = 256;
+constexpr int kMoveRows = 1;
 
-// Moves the kept rows: a thread moves one 16-byte vector of K or V.
+// Moves the kept rows of one KV head (blockIdx.y) of one sequence (blockIdx.z): a thread
+// has one 16-byte vector of K and of V in each of kMoveRows rows, all loaded before any
+// is stored.
 template <typename T, int E>
 __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
-    constexpr int VEC = 16 / sizeof(T), NV = E / VEC;
+    constexpr int VEC = 16 / sizeof(T), NV = E / VEC, PER = kMoveBlock / NV;
     wait_before();
-    const int64_t total = a.B * a.KH * a.budget * (2 * NV);
-    for (int64_t i = (int64_t)blockIdx.x * kMoveBlock + threadIdx.x; i < total; i += (int64_t)gridDim.x * kMoveBlock) {
-        const int u = (int)(i % (2 * NV));
-        int64_t r = i / (2 * NV);
-        const int at = (int)(r % a.budget);
-        r /= a.budget;
-        const int h = (int)(r % a.KH);
-        const int64_t b = r / a.KH;
-        const int slot = a.kept[r * a.budget + at];
-        if (slot < 0) continue;
-        const int64_t ho = (int64_t)h * a.c.head_stride;
-        const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot, ho);
-        const int64_t to = a.c.offset(a.new_table + b * a.new_max_pages, at, ho);
-        if (from < 0 || to < 0) continue;
-        T* pool = static_cast<T*>(u < NV ? a.k_cache : a.v_cache);
-        const int e = (u < NV ? u : u - NV) * VEC;
-        *reinterpret_cast<Vec<T, VEC>*>(pool + to + e) = *reinterpret_cast<const Vec<T, VEC>*>(pool + from + e);
+    const int64_t b = blockIdx.z;
+    const int e = threadIdx.x % NV * VEC;
+    const int at0 = blockIdx.x * (PER * kMoveRows) + threadIdx.x / NV;
+    const int64_t ho = (int64_t)blockIdx.y * a.c.head_stride;
+    const int* kept = a.kept + (b * a.KH + blockIdx.y) * a.budget;
+    const T* K = static_cast<const T*>(a.k_cache);
+    const T* V = static_cast<const T*>(a.v_cache);
+    int64_t to[kMoveRows];
+    Vec<T, VEC> x[kMoveRows], y[kMoveRows];
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+        const int at = at0 + j * PER;
+        const int slot = at < a.budget ? kept[at] : -1;
+        to[j] = -1;
+        if (slot >= 0) {
+            if (e == 0) {
+                const int64_t row = b * a.KH + blockIdx.y;
+                a.new_weights[row * a.new_slots + at] = a.weights[row * a.c.slots + slot];
+            }
+            const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot, ho);
+            if (from >= 0) {
+                to[j] = a.c.offset(a.new_table + b * a.new_max_pages, at, ho);
+                x[j] = ldg_stream<T, VEC>(K + from + e);
+                y[j] = ldg_stream<T, VEC>(V + from + e);
+            }
+        }
     }
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j)
+        if (to[j] >= 0) {
+            st_stream<T, VEC>(static_cast<T*>(a.k_cache) + to[j] + e, x[j]);
+            st_stream<T, VEC>(static_cast<T*>(a.v_cache) + to[j] + e, y[j]);
+        }
+}
+
+int launch_select(const EvictArgs& a, cudaStream_t s) {
+    int C = 1;
+    while (C < 8 && a.c.slots / C > 8192 && a.B * a.KH * C * 2 <= num_sms()) C *= 2;
+    const int most_keys = std::min(kMostKeys, (a.c.slots + C - 1) / C);
+    const size_t bytes = kHistBytes + sizeof(uint32_t) * (size_t)most_keys;
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(NNOP_ERR_CUDA, std::string("paged_evict: ") + cudaGetErrorString(e));
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.B * a.KH * C));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)C, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select, a, most_keys);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(NNOP_ERR_CUDA, std::string("paged_evict: ") + cudaGetErrorString(e));
+    }
+    return NNOP_OK;
 }
 
 template <typename T, int E>
 int launch_evict(const EvictArgs& a, cudaStream_t s) {
-    constexpr int NV = E / (16 / (int)sizeof(T));
-    evict_select<<<(unsigned)(a.B * a.KH), kSelectThreads, 0, s>>>(a);
-    if (const int rc = check_launch("paged_evict")) return rc;
-    const int64_t items = a.B * a.KH * a.budget * 2 * NV;
-    if (items == 0) return NNOP_OK;
-    const int64_t grid = std::min((items + kMoveBlock - 1) / kMoveBlock, (int64_t)1 << 30);
-    return launch_dependent("paged_evict", evict_move<T, E>, dim3((unsigned)grid), dim3(kMoveBlock), 0, s, a);
+    constexpr int kRows = kMoveBlock / (E / (16 / (int)sizeof(T))) * kMoveRows;      // per block
+    if (const int rc = launch_select(a, s)) return rc;
+    if (a.budget == 0) return NNOP_OK;
+    const unsigned grid = (unsigned)((a.budget + kRows - 1) / kRows);
+    return launch_dependent("paged_evict", evict_move<T, E>, dim3(grid, a.KH, (unsigned)a.B), dim3(kMoveBlock), 0, s, a);
 }
 
 }  // namespace
@@ -289,8 +426,9 @@ int nnop_paged_append(const void* q, const void* k, const void* v, const float* 
         if (const int rc = paged::check_cache("paged_append", a.c, block_table, lengths, E, KH, B, pages, page_size,
                                               max_pages, page_stride, head_stride, row_stride, dtype))
             return rc;
-        if (T < 0 || QH < 0 || QH > 65535 || T > ((int64_t)1 << 31) - 1024)
-            return fail(NNOP_ERR_SHAPE, "paged_append: invalid dimensions");
+        if (T < 0 || QH < 0 || QH > 65535) return fail(NNOP_ERR_SHAPE, "paged_append: invalid dimensions");
+        const int64_t most = ((int64_t)1 << 31) - 1024;
+        if (T > most || B * T > most) return fail(NNOP_ERR_SHAPE, "paged_append: more than 2^31 - 1024 new rows");
         if ((cos_t != nullptr) != (sin_t != nullptr) || (QH == 0 && q) ||
             (QH > 0 && T > 0 && B > 0 && (!q || !q_out || !cos_t)))
             return fail(NNOP_ERR_ARG, "paged_append: cos and sin come together, and q (QH > 0) with them");
@@ -311,7 +449,8 @@ int nnop_paged_append(const void* q, const void* k, const void* v, const float* 
         a.k_cache = k_cache;
         a.v_cache = v_cache;
         a.new_lengths = new_lengths;
-        a.T = T;
+        a.T = paged::FastDiv((uint32_t)std::max<int64_t>(T, 1));
+        a.tokens = B * T;
         a.B = B;
         a.cos_batch = cos_batch;
         a.QH = (int)QH;
