@@ -30,26 +30,29 @@ struct FastDiv {
 struct Cache {
     const int* table;      // [B][max_pages]
     const int* lengths;    // [B]
-    int64_t pages, max_pages;
+    uint32_t pages;
+    int64_t max_pages;
     int64_t page_stride, head_stride, row_stride;   // elements
     int slots;             // max_pages · page_size, the most a sequence can hold
     FastDiv page_size;
 
     // Tokens sequence b has cached: its length within [0, slots].
     __device__ __forceinline__ int length(int64_t b) const { return min(max(lengths[b], 0), slots); }
-    // Page and row of a slot (0 <= slot < slots) of sequence b; page < 0 where there is none.
-    __device__ __forceinline__ void place(const int* row_of_table, int slot, int64_t& page, int& row) const {
+    // A slot's entry in the table (0 <= slot < slots), and its row in that page.
+    __device__ __forceinline__ uint32_t entry(const int* row_of_table, int slot, int& row) const {
         const uint32_t i = page_size.div((uint32_t)slot);
-        row = slot - (int)(i * page_size.d);
-        const int p = __ldg(row_of_table + i);
-        page = p >= 0 && p < pages ? p : -1;
+        row = (int)((uint32_t)slot - i * page_size.d);
+        return (uint32_t)__ldg(row_of_table + i);
     }
-    // Element offset of a slot's row of head h; negative where there is no page.
-    __device__ __forceinline__ int64_t offset(const int* row_of_table, int slot, int64_t head_offset) const {
-        int64_t page;
+    // Element offset of a slot's row in a head's part of the pool; negative where there is
+    // no page.
+    __device__ __forceinline__ int64_t offset(uint32_t page, int row) const {
+        return page < pages ? page * page_stride + row * row_stride : -1;
+    }
+    __device__ __forceinline__ int64_t offset(const int* row_of_table, int slot) const {
         int row;
-        place(row_of_table, slot, page, row);
-        return page < 0 ? -1 : page * page_stride + head_offset + row * row_stride;
+        const uint32_t page = entry(row_of_table, slot, row);
+        return offset(page, row);
     }
 };
 
@@ -81,17 +84,22 @@ int guarded(const char* who, F&& body) {
 // sees them -- and none is without one.  A CTA walks its units as segments:
 // consecutive chunks of one (b, h).
 //
-// To begin and end a segment costs a CTA about what the slots of one chunk cost, so
-// where CTAs have several units each, every (b, h) counts one chunk more, an empty
-// one in front (`extra`).  Sequences of 1 to 8192 tokens, 64 of them: the slowest CTA
-// finished 17 us after the median of 157 without it (attention_mma, B200).
+// To begin and end a segment costs a CTA time too, so where CTAs have several units each
+// every (b, h) counts `kExtra` units more, empty ones in front (extra).  A CTA whose share
+// of a (b, h) is empty units alone leaves them to the next CTA.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 128;
 
+// n / d of numbers that mostly fit 32 bits.
+__device__ __forceinline__ long long div_small(long long n, long long d) {
+    if (((unsigned long long)(n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
+    return n / d;
+}
+
 struct SplitShared {
-    long long slots[kThreads / 32];
+    long long chunks[kThreads / 32];
     int some[kThreads / 32];
-    long long before;      // units / heads in front of sequence b
+    long long before;
     int b;
 };
 
@@ -99,20 +107,28 @@ struct Split {
     long long units;       // over all sequences and head tiles
     long long u, u1;       // this CTA's units left
     int G;                 // CTAs with units
-    int extra;
+    int extra;             // empty chunks in front of every (b, h)
     int b, h, chunk, chunks, len;
     long long before;      // units / heads in front of sequence b
 
-    __device__ __forceinline__ static long long start(long long units, int c, int G) { return units * c / G; }
+    __device__ __forceinline__ static long long start(long long units, int c, int G) {
+        return div_small(units * c, G);
+    }
     // The CTA that has unit e: the largest c with start(c) <= e.
-    __device__ __forceinline__ static int owner(long long units, long long e, int G) {
-        return (int)(((e + 1) * G + units - 1) / units) - 1;
+    __device__ __forceinline__ int owner(long long e) const {
+        return (int)div_small((e + 1) * G + units - 1, units) - 1;
     }
     template <int kUnit>
     __device__ __forceinline__ int chunks_of(int n) const {
         return n == 0 ? 0 : (n + kUnit - 1) / kUnit + extra;
     }
-    // Slots [first, last) of chunks c0 to c1 - 1 of this sequence.
+    // One past this CTA's last chunk of (b, h); 0: no segment is left.
+    __device__ __forceinline__ int segment() const {
+        if (u >= u1) return 0;
+        const int c1 = (int)min((long long)chunks, chunk + (u1 - u));
+        return c1 <= extra && c1 < chunks ? 0 : c1;
+    }
+    // Slots [first, end) of chunks c0 to c1 - 1 of this sequence.
     template <int kUnit>
     __device__ __forceinline__ int first_slot(int c0) const { return max(c0 - extra, 0) * kUnit; }
     template <int kUnit>
@@ -121,7 +137,7 @@ struct Split {
 
 // Block-wide (kThreads threads): the units as `ctas` CTAs share them (extra, G), and
 // part `index` of `parts` of them, set to its first unit.
-template <int kUnit>
+template <int kUnit, int kExtra>
 __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int heads, int ctas, int index, int parts,
                                              SplitShared& sh) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -146,7 +162,7 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
         }
     }
     if (lane == 31) {
-        sh.slots[warp] = incl;
+        sh.chunks[warp] = incl;
         sh.some[warp] = incl_some;
     }
     __syncthreads();
@@ -155,17 +171,17 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) {
-            before += sh.slots[w];
+            before += sh.chunks[w];
             before_some += sh.some[w];
         }
-        total += sh.slots[w];
+        total += sh.chunks[w];
         total_some += sh.some[w];
     }
     Split s;
-    s.extra = total * heads > ctas ? 1 : 0;
+    s.extra = total * heads > ctas ? kExtra : 0;
     before += s.extra * before_some;
     mine += s.extra * some;
-    s.units = (total + s.extra * total_some) * heads;
+    s.units = (total + (long long)s.extra * total_some) * heads;
     s.G = (int)min((long long)ctas, s.units);
     s.u = s.u1 = 0;
     parts = (int)min((long long)parts, s.units);
@@ -174,7 +190,7 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
         s.u1 = Split::start(s.units, index + 1, parts);
     }
     if (s.u < s.u1) {
-        const long long x = s.u / heads;      // in sequence b: before(b) <= x < before(b) + chunks(b)
+        const long long x = div_small(s.u, heads);      // in sequence b: before(b) <= x < before(b) + chunks(b)
         if (x >= before && x < before + mine) {
             int64_t b = b0;
             for (;; ++b) {
@@ -191,17 +207,22 @@ __device__ __forceinline__ Split split_begin(const Cache& c, int64_t B, int head
         s.len = c.length(s.b);
         s.chunks = s.chunks_of<kUnit>(s.len);
         const long long r = s.u - s.before * heads;
-        s.h = (int)(r / s.chunks);
-        s.chunk = (int)(r % s.chunks);
+        s.h = (int)div_small(r, s.chunks);
+        s.chunk = (int)(r - (long long)s.h * s.chunks);
+        if (s.chunk <= s.extra) {
+            s.u -= s.chunk;
+            s.chunk = 0;
+        }
     }
     return s;
 }
 
-// The next segment's (b, h) after one that ended at its last chunk.
+// On from the segment that ended at chunk c1.
 template <int kUnit>
-__device__ __forceinline__ void split_next(Split& s, const Cache& c, int heads) {
+__device__ __forceinline__ void split_next(Split& s, int c1, const Cache& c, int heads) {
+    s.u += c1 - s.chunk;
     s.chunk = 0;
-    if (++s.h < heads) return;
+    if (s.u >= s.u1 || ++s.h < heads) return;
     s.h = 0;
     do {
         s.before += s.chunks;

@@ -25,6 +25,7 @@ namespace paged {
 namespace {
 
 constexpr int kUnit = 64;          // slots per unit: 16 per warp
+constexpr int kExtra = 1;
 constexpr int kMaxCtas = 592;      // 148 SMs × 4; the workspace is sized for it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -82,12 +83,11 @@ attention_simt(AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, sub = lane & 3;
     const int heads = a.KH * a.tiles;
     let_next_start();
-    Split s = split_begin<kUnit>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
+    Split s = split_begin<kUnit, kExtra>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
-    while (s.u < s.u1) {
+    while (const int c1 = s.segment()) {
         const int c0 = s.chunk;
-        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
         const int kvh = s.h / a.tiles, r0 = (s.h % a.tiles) * R;
         const int rows = min(R, a.group - r0);
         const int qh0 = kvh * a.group + r0;
@@ -113,7 +113,7 @@ attention_simt(AttnArgs a) {
 #pragma unroll
             for (int p = 0; p < kKeys / 8; ++p) {
                 const int key = key0 + p * 8 + quad;
-                off[p] = key < end ? a.c.offset(tab, key, ho) : -1;
+                off[p] = key < end ? a.c.offset(tab, key) : -1;
                 float dot[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) dot[r] = 0.f;
@@ -122,7 +122,7 @@ attention_simt(AttnArgs a) {
                     const int vi = i * 4 + sub;
                     if (off[p] >= 0 && (NV % 4 == 0 || vi < NV)) {
                         float kv[VEC];
-                        load_vec<T, VEC>(kv, K + off[p] + vi * VEC);
+                        load_vec<T, VEC>(kv, K + ho + off[p] + vi * VEC);
 #pragma unroll
                         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -167,7 +167,7 @@ attention_simt(AttnArgs a) {
                 float vv[COLS];
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) vv[i] = 0.f;
-                if (vo >= 0 && lane * COLS < E) load_vec<T, COLS>(vv, V + vo + lane * COLS);
+                if (vo >= 0 && lane * COLS < E) load_vec<T, COLS>(vv, V + ho + vo + lane * COLS);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const float pj = __shfl_sync(0xffffffffu, p[j / 8][r], (j % 8) * 4);
@@ -211,12 +211,9 @@ attention_simt(AttnArgs a) {
                 if (e == 0) a.part_ml[slot * R + r] = make_float2(mx, sum);
             }
         }
-        s.u += c1 - c0;
-        if (!whole && c0 == 0 && threadIdx.x == 0) {
-            const long long last = s.u + (s.chunks - c1) - 1;     // the split's last unit
-            a.join[blockIdx.x] = make_int4(s.b, s.h, Split::owner(s.units, last, s.G) - blockIdx.x + 1, 0);
-        }
-        if (s.u < s.u1) split_next<kUnit>(s, a.c, heads);
+        if (!whole && c0 == 0 && threadIdx.x == 0)
+            a.join[blockIdx.x] = make_int4(s.b, s.h, s.owner(s.u + s.chunks - 1) - blockIdx.x + 1, 0);
+        split_next<kUnit>(s, c1, a.c, heads);
         __syncthreads();
     }
 }
@@ -255,22 +252,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     }
 }
 
-// W words of a row that is read once, zeros without a page.
+// W words of a row that is read once.
 template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&r)[W], const void* p, bool live) {
-    const int on = live;
-    if constexpr (W == 4) {
-        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
-                     " @p ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n}"
-                     : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]) : "l"(p), "r"(on));
-    } else if constexpr (W == 2) {
-        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n @p ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];\n}"
-                     : "=&r"(r[0]), "=&r"(r[1]) : "l"(p), "r"(on));
-    } else {
-        asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %2, 0;\n mov.b32 %0, 0;\n @p ld.global.nc.L1::no_allocate.b32 %0, [%1];\n}"
-                     : "=&r"(r[0]) : "l"(p), "r"(on));
-    }
+__device__ __forceinline__ void load_words(uint32_t (&r)[W], const char* p) {
+    if constexpr (W == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p));
+    else if constexpr (W == 2)
+        asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(p));
 }
+
+// What stands for a row that is not there: a finite V, so that its weight of 0 counts.
+__device__ const uint4 no_row[16] = {};
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -292,22 +287,32 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     }
 }
 
+#ifndef EXTRA
+#define EXTRA 8
+#endif
+#ifndef C1
+#define C1 3
+#endif
+#ifndef C2
+#define C2 2
+#endif
 template <int E> struct MmaShape {
     static constexpr int kTiles = E >= 128 ? 1 : E == 64 ? 2 : 4;   // 16-key tiles a warp takes at once (8 KB of K and V from E = 32)
     static constexpr int kKeys = 16 * kTiles;
-    static constexpr int kUnit = 4 * kKeys;                         // slots per unit
+    static constexpr int kUnit = kKeys;                             // slots per unit of the split
+    static constexpr int kExtra = EXTRA;
 };
 
 // CTAs per SM.  What has to be in flight to keep HBM busy lies in registers, 8 KB a
 // warp, beside 32·NT for Oᵀ and 16·NT for Q: three CTAs of 168 registers a thread
 // (181 us for 64 sequences up to 8192) before two of 255 (194 us) or four that spill
 // (236 us); with two head tiles a warp, two.
-constexpr int mma_ctas(int NT) { return NT == 1 ? 3 : 2; }
+constexpr int mma_ctas(int E, int NT) { return NT == 1 ? C1 : C2; }
 
 // NT: head tiles (of 8) per warp, which share the fragments of K and V.  WT: warps
 // that read the same keys for other head tiles; 4/WT warps share the keys out.
 template <typename T, int E, int NT, int WT, bool kWholeTiles>
-__global__ void __launch_bounds__(kThreads, mma_ctas(NT))
+__global__ void __launch_bounds__(kThreads, mma_ctas(E, NT))
 attention_mma(AttnArgs a) {
     using S = MmaShape<E>;
     constexpr int R = 8 * NT * WT;
@@ -320,89 +325,145 @@ attention_mma(AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, sub = lane & 3;
     const int tile0 = warp % WT * NT, part = warp / WT;
     const int heads = a.KH * a.tiles;
-    const T* K = static_cast<const T*>(a.k);
-    const T* V = static_cast<const T*>(a.v);
     let_next_start();
-    Split s = split_begin<S::kUnit>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
+    Split s = split_begin<S::kUnit, S::kExtra>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
-    while (s.u < s.u1) {
-        const int c0 = s.chunk;
-        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
-        const int kvh = s.h / a.tiles, r0 = (s.h % a.tiles) * R;
-        const int rows = min(R, a.group - r0);
-        const int qh0 = kvh * a.group + r0;
-        const int* tab = a.c.table + (int64_t)s.b * a.c.max_pages;
-        const int64_t ho = (int64_t)kvh * a.c.head_stride;
-        // Q: B fragments of all k16 steps; head gid of each of this warp's tiles
-        uint32_t q[NT][KC][KW];
-        float m[NT][2], l[NT][2], acc[NT][VC][VW][4];
+    int c1 = s.segment();
+    if (c1 == 0) return;
+
+    int rows, qh0, end, key0;
+    const int* tab;
+    uint32_t q[NT][KC][KW];        // B fragments of all k16 steps; head gid of each of this warp's tiles
+    uint32_t kr[S::kTiles][2][KC][KW], vr[S::kTiles][4][VC][VW];
+    const char *kl, *vl;           // this head's pools, at this lane's first row and bytes of a tile
+    // Bytes between a lane's rows: K 8 rows on; V 1, 8 and 9 rows on.
+    const int64_t rs = a.c.row_stride * 2;
+    constexpr int kStep = S::kKeys * (4 / WT);
+
+    // Where a step's rows are.  kWholeTiles (pages of a multiple of 16 slots): a tile of 16
+    // keys lies in one page, one lookup for all lanes, made a step ahead (168 us for 64
+    // sequences up to 8192; 175 when it is made with the loads).  Else one lookup for each
+    // row a lane reads (pages of 20: 191 us; a step ahead in other lanes and handed out by
+    // shuffles: 221).
+    uint32_t page[S::kTiles];      // table entries of the next step's tiles
+    int row[S::kTiles];
+    int64_t tiles[S::kTiles];      // bytes into the pool; negative: no page
+    bool inside;                   // all of the step's keys have rows
+    auto find = [&](int key0) {
+        if constexpr (kWholeTiles) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+                page[t] = key0 + t * 16 < end ? a.c.entry(tab, key0 + t * 16, row[t]) : ~0u;
+        }
+    };
+    auto found = [&](int key0) {
+        inside = kWholeTiles && key0 + S::kKeys <= end;
+        if constexpr (kWholeTiles) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) {
+                tiles[t] = a.c.offset(page[t], row[t]) * 2;
+                inside = inside && tiles[t] >= 0;
+            }
+        }
+    };
+    // Bytes into the pool of key + mine of tile t, counted from where kl and vl point.
+    auto row_at = [&](int t, int key, int mine, int first) -> int64_t {
+        if (key + mine >= end) return -1;
+        if constexpr (kWholeTiles) return tiles[t] < 0 ? -1 : tiles[t] + (mine - first) * rs;
+        const int64_t x = a.c.offset(tab, key + mine);
+        return x < 0 ? -1 : x * 2;
+    };
+    // K of the step at key0; bit 2t + i: this lane's key 16t + 8i + gid has a row.
+    auto load_k = [&](int key0) -> uint32_t {
+        if (inside) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], kl + tiles[t] + i * 8 * rs + c * (16 * KW));
+            return ~0u;
+        }
+        uint32_t has = 0;
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t x = row_at(t, key0 + t * 16, i * 8 + gid, gid);
+                has |= (uint32_t)(x >= 0) << (2 * t + i);
+                const char* p = x >= 0 ? kl + x : reinterpret_cast<const char*>(no_row);
+#pragma unroll
+                for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], p + c * (16 * KW));
+            }
+        return has;
+    };
+    auto load_v = [&](int key0) {
+        if (inside) {
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+                        load_words<VW>(vr[t][i][c], vl + tiles[t] + ((i >> 1) * 8 + (i & 1)) * rs + c * (32 * VW));
+            return;
+        }
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t x = row_at(t, key0 + t * 16, (i >> 1) * 8 + (i & 1) + 2 * sub, 2 * sub);
+                const char* p = x >= 0 ? vl + x : reinterpret_cast<const char*>(no_row);
+#pragma unroll
+                for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], p + c * (32 * VW));
+            }
+    };
+    uint32_t live = 0;
+    // The segment [s.chunk, c1) of (s.b, s.h): its Q, and the first step's K and V.
+    auto enter = [&]() {
+        const int kvh = s.h / a.tiles, r0 = (s.h - kvh * a.tiles) * R;
+        rows = min(R, a.group - r0);
+        qh0 = kvh * a.group + r0;
+        tab = a.c.table + (int64_t)s.b * a.c.max_pages;
+        kl = static_cast<const char*>(a.k) + kvh * a.c.head_stride * 2 + sub * (4 * KW) + (kWholeTiles ? gid * rs : 0);
+        vl = static_cast<const char*>(a.v) + kvh * a.c.head_stride * 2 + gid * (4 * VW) + (kWholeTiles ? 2 * sub * rs : 0);
+        end = s.end_slot<S::kUnit>(c1);
+        key0 = s.first_slot<S::kUnit>(s.chunk) + part * S::kKeys;
+        find(key0);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = (tile0 + n) * 8 + gid;
-            const T* row = static_cast<const T*>(a.q) + ((int64_t)s.b * a.QH + qh0 + r) * E;
+            const char* row = r < rows ? static_cast<const char*>(a.q) + ((int64_t)s.b * a.QH + qh0 + r) * (2 * E) + sub * (4 * KW)
+                                       : reinterpret_cast<const char*>(no_row);
 #pragma unroll
-            for (int c = 0; c < KC; ++c) load_words<KW>(q[n][c], row + (c * 4 + sub) * (2 * KW), r < rows);
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.f;
+            for (int c = 0; c < KC; ++c) load_words<KW>(q[n][c], row + c * (16 * KW));
+        }
+        if (key0 < end) {
+            found(key0);
+            live = load_k(key0);
+            load_v(key0);
+            find(key0 + kStep);
+        }
+    };
+    enter();
+    for (;;) {
+        // running maximum of the raw scores of heads 2·sub and 2·sub + 1, what the weights are
+        // relative to (log2), this lane's sum of weights, Oᵀ
+        float m[NT][2], base[NT][2], l[NT][2], acc[NT][VC][VW][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                m[n][j] = -INFINITY;
+                base[n][j] = l[n][j] = 0.f;
+            }
 #pragma unroll
             for (int c = 0; c < VC; ++c)
 #pragma unroll
                 for (int j = 0; j < VW; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[n][c][j][i] = 0.f;
-        }
-        const int end = s.end_slot<S::kUnit>(c1);
-        uint32_t kr[S::kTiles][2][KC][KW], vr[S::kTiles][4][VC][VW];
-        uint32_t live = 0;             // bit 2t + i: this lane's key 16t + 8i + gid has a row
-        // Where a step's rows are (negative offset: no row).  kWholeTiles (pages of a multiple
-        // of 16 slots): a tile of 16 keys lies in one page, one lookup for all lanes, made a
-        // step ahead (168 us for 64 sequences up to 8192; 175 when it is made with the loads).
-        // Else one lookup for each row a lane reads (pages of 20: 191 us; a step ahead in
-        // other lanes and handed out by shuffles: 221).
-        int64_t tiles[S::kTiles];
-        auto find = [&](int key0) {
-            if constexpr (kWholeTiles) {
-#pragma unroll
-                for (int t = 0; t < S::kTiles; ++t)
-                    tiles[t] = key0 + t * 16 < end ? a.c.offset(tab, key0 + t * 16, ho) : -1;
-            }
-        };
-        auto row_at = [&](int t, int key, int mine) -> int64_t {
-            if (key + mine >= end) return -1;
-            if constexpr (kWholeTiles) return tiles[t] < 0 ? -1 : tiles[t] + mine * a.c.row_stride;
-            return a.c.offset(tab, key + mine, ho);
-        };
-        auto load_k = [&](int key0) {
-            uint32_t has = 0;
-#pragma unroll
-            for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int64_t x = row_at(t, key0 + t * 16, i * 8 + gid);
-                    has |= (uint32_t)(x >= 0) << (2 * t + i);
-#pragma unroll
-                    for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], K + x + (c * 4 + sub) * (2 * KW), x >= 0);
-                }
-            return has;
-        };
-        auto load_v = [&](int key0) {
-#pragma unroll
-            for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t x = row_at(t, key0 + t * 16, (i >> 1) * 8 + (i & 1) + 2 * sub);
-#pragma unroll
-                    for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], V + x + (c * 8 + gid) * (2 * VW), x >= 0);
-                }
-        };
-        constexpr int kStep = S::kKeys * (4 / WT);
-        int key0 = s.first_slot<S::kUnit>(c0) + part * S::kKeys;
-        if (key0 < end) {
-            find(key0);
-            live = load_k(key0);
-            load_v(key0);
-            find(key0 + kStep);
         }
         for (; key0 < end; key0 += kStep) {
             float d[NT][S::kTiles][4];
@@ -420,57 +481,68 @@ attention_mma(AttnArgs a) {
                                         q[n][c][w], q[n][c][w + 1]);
                 }
             const bool more = key0 + kStep < end;
-            const uint32_t next = more ? load_k(key0 + kStep) : 0;
-            // scores to weights against the running maximum; heads 2·sub and 2·sub + 1
+            uint32_t next = 0;
+            if (more) {
+                found(key0 + kStep);
+                next = load_k(key0 + kStep);
+            }
+            if (live != ~0u) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(live >> (2 * t + i / 2) & 1)) d[n][t][i] = -INFINITY;
+            }
+            if (a.scores != nullptr) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = key0 + t * 16 + i / 2 * 8 + gid, r = (tile0 + n) * 8 + 2 * sub + i % 2;
+                            if (key < end && r < rows)
+                                a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = d[n][t][i] * a.scale2;
+                        }
+            }
             uint32_t b[NT][S::kTiles][2][2];      // Pᵀ: [16-bit term][key half]
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float mx[2] = {m[n][0], m[n][1]};
+                float mx[2] = {d[n][0][0], d[n][0][1]};
 #pragma unroll
-                for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int at = t * 16 + i * 8;
-                        const bool on = live >> (2 * t + i) & 1;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            float& x = d[n][t][i * 2 + j];
-                            x = on ? x * a.scale2 : -INFINITY;
-                            mx[j] = fmaxf(mx[j], x);
-                            const int key = key0 + at + gid, r = (tile0 + n) * 8 + 2 * sub + j;
-                            if (a.scores != nullptr && key < end && r < rows)
-                                a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = x;
-                        }
-                    }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+                for (int t = 0; t < S::kTiles; ++t) {
+                    mx[0] = fmaxf(mx[0], fmaxf(d[n][t][0], d[n][t][2]));
+                    mx[1] = fmaxf(mx[1], fmaxf(d[n][t][1], d[n][t][3]));
                 }
-                float base[2];
+                // the maximum rises only now and then: the lanes meet only when one of them has more
+                if (__any_sync(0xffffffffu, mx[0] > m[n][0] || mx[1] > m[n][1])) {
+                    float f[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) base[j] = mx[j] == -INFINITY ? 0.f : mx[j] - kShift;    // -Inf: no score yet
-                if (__any_sync(0xffffffffu, mx[0] != m[n][0] || mx[1] != m[n][1])) {
-                    const float f0 = fast_exp2(m[n][0] - kShift - base[0]), f1 = fast_exp2(m[n][1] - kShift - base[1]);
-                    l[n][0] *= f0;
-                    l[n][1] *= f1;
+                    for (int j = 0; j < 2; ++j) {
+                        mx[j] = fmaxf(mx[j], m[n][j]);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
+                        const float to = mx[j] == -INFINITY ? 0.f : mx[j] * a.scale2 - kShift;    // -Inf: no score yet
+                        f[j] = m[n][j] == -INFINITY ? 0.f : fast_exp2(base[n][j] - to);
+                        m[n][j] = mx[j];
+                        base[n][j] = to;
+                        l[n][j] *= f[j];
+                    }
 #pragma unroll
                     for (int c = 0; c < VC; ++c)
 #pragma unroll
-                        for (int j = 0; j < VW; ++j) {
-                            acc[n][c][j][0] *= f0;
-                            acc[n][c][j][1] *= f1;
-                            acc[n][c][j][2] *= f0;
-                            acc[n][c][j][3] *= f1;
-                        }
-                    m[n][0] = mx[0];
-                    m[n][1] = mx[1];
+                        for (int j = 0; j < VW; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[n][c][j][i] *= f[i & 1];
                 }
 #pragma unroll
                 for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float p0 = fast_exp2(d[n][t][i * 2] - base[0]), p1 = fast_exp2(d[n][t][i * 2 + 1] - base[1]);
+                        const float p0 = fast_exp2(fmaf(d[n][t][i * 2], a.scale2, -base[n][0]));
+                        const float p1 = fast_exp2(fmaf(d[n][t][i * 2 + 1], a.scale2, -base[n][1]));
                         l[n][0] += p0;
                         l[n][1] += p1;
                         float e0, e1, u0, u1;
@@ -498,7 +570,15 @@ attention_mma(AttnArgs a) {
             live = next;
             find(key0 + 2 * kStep);
         }
-        // join the warps of each head tile
+        // The next segment's first loads go out before this one's warps are joined.
+        const bool first = s.chunk == 0, whole = first && c1 == s.chunks;
+        const int slot = 2 * blockIdx.x + (first ? 1 : 0);
+        const int b_of = s.b, rows_of = rows, qh_of = qh0;
+        if (!whole && first && threadIdx.x == 0)
+            a.join[blockIdx.x] = make_int4(s.b, s.h, s.owner(s.u + s.chunks - 1) - blockIdx.x + 1, 0);
+        split_next<S::kUnit>(s, c1, a.c, heads);
+        c1 = s.segment();
+        if (c1 != 0) enter();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -506,7 +586,7 @@ attention_mma(AttnArgs a) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], o);
                 if (gid == 0) {
-                    wm[warp][n * 8 + 2 * sub + j] = m[n][j] - kShift;
+                    wm[warp][n * 8 + 2 * sub + j] = m[n][j] == -INFINITY ? -INFINITY : base[n][j];
                     wl[warp][n * 8 + 2 * sub + j] = l[n][j];
                 }
             }
@@ -520,9 +600,7 @@ attention_mma(AttnArgs a) {
                             make_float2(acc[n][c][j][h], acc[n][c][j][2 + h]);
         }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == s.chunks;
-        const int slot = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
-        for (int i = threadIdx.x; i < rows * E; i += kThreads) {
+        for (int i = threadIdx.x; i < rows_of * E; i += kThreads) {
             const int r = i / E, e = i % E;
             float mw[4 / WT], mx = -INFINITY;
 #pragma unroll
@@ -539,144 +617,139 @@ attention_mma(AttnArgs a) {
                 ac = fmaf(wacc[w * WT + r / (8 * NT)][r % (8 * NT)][e], f, ac);
             }
             if (whole) {
-                write_row<T, E>(a, s.b, qh0 + r, e, ac, mx, sum);
+                write_row<T, E>(a, b_of, qh_of + r, e, ac, mx, sum);
             } else {
                 a.part_acc[((int64_t)slot * R + r) * E + e] = ac;
                 if (e == 0) a.part_ml[slot * R + r] = make_float2(mx, sum);
             }
         }
-        s.u += c1 - c0;
-        if (!whole && c0 == 0 && threadIdx.x == 0) {
-            const long long last = s.u + (s.chunks - c1) - 1;     // the split's last unit
-            a.join[blockIdx.x] = make_int4(s.b, s.h, Split::owner(s.units, last, s.G) - blockIdx.x + 1, 0);
-        }
-        if (s.u < s.u1) split_next<S::kUnit>(s, a.c, heads);
+        if (c1 == 0) return;
         __syncthreads();
     }
 }
 
-// What the parts of one row come to: maximum (log2 domain) and sum.  A warp; part i lies
-// in slot 2(c + i), the first in 2c + 1.
-__device__ __forceinline__ float2 join_ml(const float2* part_ml, int R, int c, int parts, int r) {
-    const int lane = threadIdx.x & 31;
-    float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < parts; i += 32) {
-        const float2 ml = part_ml[(2 * (c + i) + (i == 0 ? 1 : 0)) * R + r];
-        const float mx = fmaxf(m, ml.x), base = mx == -INFINITY ? 0.f : mx;
-        l = l * fast_exp2(m - base) + ml.y * fast_exp2(ml.x - base);
-        m = mx;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-        const float mx = fmaxf(m, m2), base = mx == -INFINITY ? 0.f : mx;
-        l = l * fast_exp2(m - base) + l2 * fast_exp2(m2 - base);
-        m = mx;
-    }
-    return make_float2(m, l);
+// Joins two parts of a row: maximum (log2 domain), sum and what is weighed with them.
+__device__ __forceinline__ float2 join_two(float2 x, float2 y, float& fx, float& fy) {
+    const float mx = fmaxf(x.x, y.x), base = mx == -INFINITY ? 0.f : mx;
+    fx = fast_exp2(x.x - base);
+    fy = fast_exp2(y.x - base);
+    return make_float2(mx, x.y * fx + y.y * fy);
 }
 
-constexpr int kJoinThreads = 128;
+// Part i of a split that CTA c has the first part of lies in slot 2(c + i), the first in 2c + 1.
+__device__ __forceinline__ int part_slot(int c, int i) { return 2 * (c + i) + (i == 0 ? 1 : 0); }
 
-// Second launch.  Blocks below rows·ctas: row blockIdx.x mod rows of the (sequence,
-// head tile) whose first part CTA blockIdx.x / rows wrote.  The others (with weights):
-// weights[b][kv head][j] += Σ over the group of exp(s_j − lse) for a share of the
-// slots; a split row's lse comes from its parts again, so that both run at once.
-template <typename T, int E, int R, int kUnit>
-__global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs a, int rows, int ctas) {
+// log2 of the sum of a row's parts, by a warp.
+__device__ __forceinline__ float join_lse2(const float2* part_ml, int R, int c, int parts, int r) {
+    const int lane = threadIdx.x & 31;
+    float2 x = make_float2(-INFINITY, 0.f);
+    float f0, f1;
+    for (int i = lane; i < parts; i += 32) x = join_two(x, part_ml[part_slot(c, i) * R + r], f0, f1);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        x = join_two(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)), f0, f1);
+    return x.y > 0.f || x.y != x.y ? x.x + log2f(x.y) : -INFINITY;
+}
+
+// Second launch.  The last rows·ctas blocks: row j mod rows of the (sequence, head tile)
+// whose first part CTA j / rows wrote, each group of E/4 threads taking some of the
+// parts.  The `adders` blocks in front (with weights): weights[b][kv head][j] += Σ over the
+// group of exp(s_j − lse) for a share of the slots; a split row's lse comes from its
+// parts again, so that both run at once.
+template <typename T, int E, int R, int kUnit, int kExtra>
+__global__ void __launch_bounds__(kThreads) attention_join(AttnArgs a, int rows, int ctas, int adders) {
     constexpr int LE = E / 4;                             // lanes per row of 16-byte vectors
-    constexpr int NP = kJoinThreads / LE;                 // parts at once
+    constexpr int NP = kThreads / LE;                     // parts at once
     __shared__ __align__(16) union {
-        float acc[NP][E];
+        struct {
+            float acc[NP][E];
+            float2 ml[NP];
+        } j;
         struct {
             SplitShared split;
             float lse2[32];
         } w;
     } sh;
-    static_assert(kThreads == kJoinThreads, "split_begin counts on kThreads threads");
-    wait_before();
     const int t = threadIdx.x;
-    if ((int)blockIdx.x < rows * ctas) {
-        const int c = blockIdx.x / rows, r = blockIdx.x % rows;
+    if ((int)blockIdx.x >= adders) {
+        wait_before();
+        const int c = (blockIdx.x - adders) / rows, r = (blockIdx.x - adders) % rows;
         const int4 w = a.join[c];
         const int r0 = (w.y % a.tiles) * R;
         if (w.z == 0 || r0 + r >= a.group) return;
-        const float2 ml = join_ml(a.part_ml, R, c, w.z, r);
-        const float base = ml.x == -INFINITY ? 0.f : ml.x;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        float f0, f1;
 #pragma unroll 4
         for (int i = t / LE; i < w.z; i += NP) {
-            const int slot = 2 * (c + i) + (i == 0 ? 1 : 0);
-            const float f = fast_exp2(a.part_ml[slot * R + r].x - base);
+            const int slot = part_slot(c, i);
             const float4 y = *reinterpret_cast<const float4*>(a.part_acc + ((int64_t)slot * R + r) * E + (t % LE) * 4);
-            x.x = fmaf(f, y.x, x.x);
-            x.y = fmaf(f, y.y, x.y);
-            x.z = fmaf(f, y.z, x.z);
-            x.w = fmaf(f, y.w, x.w);
+            ml = join_two(ml, a.part_ml[slot * R + r], f0, f1);
+            x.x = x.x * f0 + y.x * f1;
+            x.y = x.y * f0 + y.y * f1;
+            x.z = x.z * f0 + y.z * f1;
+            x.w = x.w * f0 + y.w * f1;
         }
-        *reinterpret_cast<float4*>(&sh.acc[t / LE][(t % LE) * 4]) = x;
+        *reinterpret_cast<float4*>(&sh.j.acc[t / LE][(t % LE) * 4]) = x;
+        if (t % LE == 0) sh.j.ml[t / LE] = ml;
         __syncthreads();
         if (t < E) {
-            float sum = 0.f;
+            float sum = sh.j.acc[0][t];
+            ml = sh.j.ml[0];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) sum += sh.acc[i][t];
+            for (int i = 1; i < NP; ++i) {
+                ml = join_two(ml, sh.j.ml[i], f0, f1);
+                sum = sum * f0 + sh.j.acc[i][t] * f1;
+            }
             write_row<T, E>(a, w.x, (w.y / a.tiles) * a.group + r0 + r, t, sum, ml.x, ml.y);
         }
         return;
     }
-    // The first launch's split again.  Head tile h of sequence b has units
-    // [before·heads + h·chunks, ... + chunks), so which CTAs had them is known.
-    Split s = split_begin<kUnit>(a.c, a.B, a.KH * a.tiles, ctas, blockIdx.x - rows * ctas, gridDim.x - rows * ctas, sh.w.split);
-    const long long units = s.units;
-    const int G = s.G;
-    while (s.u < s.u1) {
-        const int c0 = s.chunk;
-        const int c1 = (int)min((long long)s.chunks, c0 + (s.u1 - s.u));
+    // The first launch's split again, which rests on the call's arguments alone.
+    const int heads = a.KH * a.tiles;
+    Split s = split_begin<kUnit, kExtra>(a.c, a.B, heads, ctas, blockIdx.x, adders, sh.w.split);
+    wait_before();
+    while (const int c1 = s.segment()) {
         const int end = s.end_slot<kUnit>(c1);
         const int kvh = s.h / a.tiles;
-        // a chunk's weights are added up by the CTA that has it for the first head tile
+        // a chunk's weights are added up by the block that has it for the first head tile
         if (s.h % a.tiles == 0) {
             const int64_t row0 = (int64_t)s.b * a.QH + kvh * a.group;
             float* w = a.weights + ((int64_t)s.b * a.KH + kvh) * a.c.slots;
             for (int g0 = 0; g0 < a.group; g0 += 32) {
+                const int n = min(32, a.group - g0);
                 __syncthreads();
-                for (int g = t / 32; g < min(32, a.group - g0); g += kJoinThreads / 32) {
+                for (int g = t / 32; g < n; g += kThreads / 32) {
                     const int tile = (g0 + g) / R, r = (g0 + g) % R;
-                    const long long u = (s.before * a.KH * a.tiles) + (long long)(s.h + tile) * s.chunks;
-                    const int first = Split::owner(units, u, G), last = Split::owner(units, u + s.chunks - 1, G);
-                    float lse2;
-                    if (first == last) {
-                        lse2 = a.lse[row0 + g0 + g] * kLog2e;
-                    } else {
-                        const float2 ml = join_ml(a.part_ml, R, first, last - first + 1, r);
-                        lse2 = ml.y > 0.f || ml.y != ml.y ? ml.x + log2f(ml.y) : -INFINITY;
-                    }
+                    // head tile h of sequence b has units before·heads + h·chunks + [0, chunks)
+                    const long long u = s.before * heads + (long long)(s.h + tile) * s.chunks;
+                    const int first = s.owner(u + s.extra), last = s.owner(u + s.chunks - 1);
+                    const float lse2 = first == last ? a.lse[row0 + g0 + g] * kLog2e
+                                                     : join_lse2(a.part_ml, R, first, last - first + 1, r);
                     if (t % 32 == 0) sh.w.lse2[g] = lse2;
                 }
                 __syncthreads();
                 // four slots a thread at once: their loads do not wait for one another
-                const int heads = min(32, a.group - g0);
-                for (int j0 = s.first_slot<kUnit>(c0) + t; j0 < end; j0 += 4 * kJoinThreads) {
+                for (int j0 = s.first_slot<kUnit>(s.chunk) + t; j0 < end; j0 += 4 * kThreads) {
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    for (int g = 0; g < heads; ++g) {
+                    for (int g = 0; g < n; ++g) {
                         const float lse2 = sh.w.lse2[g];
                         const float* sc = a.scores + (row0 + g0 + g) * a.c.slots;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int j = j0 + i * kJoinThreads;
+                            const int j = j0 + i * kThreads;
                             if (j < end && lse2 != -INFINITY) sum[i] += fast_exp2(sc[j] - lse2);
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int j = j0 + i * kJoinThreads;
+                        const int j = j0 + i * kThreads;
                         if (j < end) w[j] += sum[i];
                     }
                 }
             }
         }
-        s.u += c1 - c0;
-        if (s.u < s.u1) split_next<kUnit>(s, a.c, a.KH * a.tiles);
+        split_next<kUnit>(s, c1, a.c, heads);
     }
 }
 
@@ -720,16 +793,17 @@ int launch(const AttnArgs& a, cudaStream_t s) {
         attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
     } else {
         constexpr int NT = R == 8 ? 1 : 2, WT = R / (8 * NT);
-        G = std::min(kMaxCtas, mma_ctas(NT) * num_sms());
+        G = std::min(kMaxCtas, mma_ctas(E, NT) * num_sms());
         if (a.c.page_size.d % 16 == 0)
             attention_mma<T, E, NT, WT, true><<<G, kThreads, 0, s>>>(a);
         else
             attention_mma<T, E, NT, WT, false><<<G, kThreads, 0, s>>>(a);
     }
     if (const int rc = check_launch("paged_attention")) return rc;
-    const int rows = std::min(R, a.group);
-    return launch_dependent("paged_attention", attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit>,
-                            dim3(G * rows + (a.weights != nullptr ? 8 * num_sms() : 0)), dim3(kJoinThreads), 0, s, a, rows, G);
+    const int rows = std::min(R, a.group), adders = a.weights != nullptr ? 8 * num_sms() : 0;
+    return launch_dependent("paged_attention",
+                            attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit, f32 ? kExtra : MmaShape<E>::kExtra>,
+                            dim3(adders + G * rows), dim3(kThreads), 0, s, a, rows, G, adders);
 }
 
 template <typename T, int E>

@@ -40,7 +40,7 @@ int check_cache(const char* who, Cache& c, const int32_t* table, const int32_t* 
     if (B > 0 && (!lengths || (max_pages > 0 && !table))) return fail(NNOP_ERR_ARG, w + ": NULL pointer");
     c.table = table;
     c.lengths = lengths;
-    c.pages = pages;
+    c.pages = (uint32_t)pages;
     c.max_pages = max_pages;
     c.page_stride = page_stride;
     c.head_stride = head_stride;
@@ -106,9 +106,9 @@ __global__ void __launch_bounds__(kAppendBlock) append_kernel(AppendArgs a) {
     } else {
         const int64_t slot = (int64_t)a.c.length(b) + t;
         if ((a.n_new && t >= a.n_new[b]) || slot >= a.c.slots) return;
-        const int64_t to = a.c.offset(a.c.table + b * a.c.max_pages, (int)slot, (int64_t)h0 * a.c.head_stride);
+        const int64_t to = a.c.offset(a.c.table + b * a.c.max_pages, (int)slot);
         if (to < 0) return;
-        dst = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + to + u * VEC;
+        dst = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + to + h0 * a.c.head_stride + u * VEC;
         dst_step = a.c.head_stride;
     }
     Vec<T, VEC> x[kAppendHeads], y[kAppendHeads];
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
     const int64_t b = blockIdx.z;
     const int e = threadIdx.x % NV * VEC;
     const int at0 = blockIdx.x * (PER * kMoveRows) + threadIdx.x / NV;
-    const int64_t ho = (int64_t)blockIdx.y * a.c.head_stride;
+    const int64_t ho = blockIdx.y * a.c.head_stride + e;
     const int* kept = a.kept + (b * a.KH + blockIdx.y) * a.budget;
     const T* K = static_cast<const T*>(a.k_cache);
     const T* V = static_cast<const T*>(a.v_cache);
@@ -345,19 +345,19 @@ __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
                 const int64_t row = b * a.KH + blockIdx.y;
                 a.new_weights[row * a.new_slots + at] = a.weights[row * a.c.slots + slot];
             }
-            const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot, ho);
+            const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot);
             if (from >= 0) {
-                to[j] = a.c.offset(a.new_table + b * a.new_max_pages, at, ho);
-                x[j] = ldg_stream<T, VEC>(K + from + e);
-                y[j] = ldg_stream<T, VEC>(V + from + e);
+                to[j] = a.c.offset(a.new_table + b * a.new_max_pages, at);
+                x[j] = ldg_stream<T, VEC>(K + from + ho);
+                y[j] = ldg_stream<T, VEC>(V + from + ho);
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j)
         if (to[j] >= 0) {
-            st_stream<T, VEC>(static_cast<T*>(a.k_cache) + to[j] + e, x[j]);
-            st_stream<T, VEC>(static_cast<T*>(a.v_cache) + to[j] + e, y[j]);
+            st_stream<T, VEC>(static_cast<T*>(a.k_cache) + to[j] + ho, x[j]);
+            st_stream<T, VEC>(static_cast<T*>(a.v_cache) + to[j] + ho, y[j]);
         }
 }
 

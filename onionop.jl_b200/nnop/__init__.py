@@ -26,6 +26,8 @@ position_ids (L, B)            position_ids (B, L) float32
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ._lib import (BF16, F16, F32, NNopError, NNopShapeError, check, lib)
@@ -691,50 +693,61 @@ def llama_rope(q, k, *, cos, sin):
 # whole sequences: the step after it, one new token against the cached ones)
 # =========================================================================
 
-# These run once per generated token, where the host's time counts: plain checks, and
-# the device as its index (-1 on the CPU).
+# These run once per generated token and layer, where the host's time is most of a small
+# call's: plain checks in the order of a valid call, the device as its index (-1 on the
+# CPU), messages made only when they are needed.
 
-def _paged_dims(name, k_cache, v_cache, block_table, lengths, others, write):
-    """Checks of the cache arguments the paged calls share; returns the device's
-    index, the batch and ``(pages, page_size, max_pages, strides...)`` as the C ABI
-    takes them."""
-    dev = k_cache.get_device()
-    for t in (k_cache, v_cache, block_table, lengths, *others):
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.nnop_paged_attention_fwd_workspace_size)
+
+
+def _paged_device(name, *ts):
+    """Index of the CUDA device that all of ts (None allowed) are on."""
+    dev = ts[0].get_device()
+    for t in ts:
         if t is not None and (dev < 0 or t.get_device() != dev):
-            if not (k_cache.is_cuda and t.is_cuda):
+            if not (ts[0].is_cuda and t.is_cuda):
                 raise NNopError(-3, "nnop operates on CUDA tensors only (no CPU fallback)")
             raise NNopError(-3, f"{name}: all tensors must be on one device")
+    return dev
+
+
+def _paged_dims(name, k_cache, v_cache, block_table, lengths, write):
+    """Checks of the cache arguments the paged calls share; returns the batch, KH, E
+    and ``(pages, page_size, max_pages, strides...)`` as the C ABI takes them."""
     shape = k_cache.shape
     if len(shape) != 4 or shape != v_cache.shape:
         raise NNopShapeError(-1, f"{name}: k_cache and v_cache must be 4-d (P, KH, PS, E) of one shape")
-    if k_cache.dtype != v_cache.dtype:
+    if k_cache.dtype is not v_cache.dtype:
         raise NNopError(-2, f"{name}: k_cache and v_cache must share a dtype")
+    if block_table.dtype is not torch.int32 or lengths.dtype is not torch.int32:
+        raise NNopError(-2, f"{name}: block_table and lengths must be int32")
     tshape, nshape = block_table.shape, lengths.shape
     if len(tshape) != 2 or len(nshape) != 1 or tshape[0] != nshape[0]:
         raise NNopShapeError(-1, f"{name}: block_table must be (B, MP) and lengths (B,)")
-    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
-        raise NNopError(-2, f"{name}: block_table and lengths must be int32")
-    strides = k_cache.stride()
-    if min(shape) <= 1 or strides != v_cache.stride():     # the stride of an axis of length 1 means nothing
-        strides, sv = (tuple(st if n > 1 else 0 for n, st in zip(shape, t.stride())) for t in (k_cache, v_cache))
-        if strides[:3] != sv[:3]:
+    P, KH, PS, E = shape
+    sp, sh, sr, se = strides = k_cache.stride()
+    if P <= 1 or KH <= 1 or PS <= 1 or strides != v_cache.stride():   # the stride of an axis of length 1 means nothing
+        (sp, sh, sr), sv = (tuple(st if n > 1 else 0 for n, st in zip((P, KH, PS), t.stride())) for t in (k_cache, v_cache))
+        if (sp, sh, sr) != sv:
             raise NNopShapeError(-1, f"{name}: k_cache and v_cache must have the same strides")
-    if shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        se = se if v_cache.stride(3) == 1 else 0
+    if se != 1 and E > 1:
         raise NNopShapeError(-1, f"{name}: the caches' embedding axis must be contiguous")
-    if write and any(st == 0 and n > 1 for n, st in zip(shape, strides)):
+    if write and ((sp == 0 and P > 1) or (sh == 0 and KH > 1) or (sr == 0 and PS > 1)):
         raise NNopShapeError(-1, f"{name}: an expanded cache cannot be written")
-    return dev, nshape[0], (shape[0], shape[2], tshape[1], strides[0], strides[1], strides[2])
+    return nshape[0], KH, E, (P, PS, tshape[1], sp, sh, sr)
 
 
 def _no_grad(name, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise NNopError(-3, f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise NNopError(-3, f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _aligned(t):
     """Contiguous and on a 16-byte boundary (a view may start off one)."""
-    if t is None:
-        return None
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -742,42 +755,50 @@ def _aligned(t):
 def _on(dev, fn, *args):
     """Calls the library on device ``dev`` with its current stream last."""
     if dev == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+        status = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        check(status)
 
 
 def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, sin, n_new):
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (q, k, v, cos, sin, n_new), True)
+    dev = _paged_device(name, k_cache, v_cache, block_table, lengths, k, v, q, cos, sin, n_new)
+    B, KH, E, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, True)
     _no_grad(name, q, k, v, k_cache, v_cache)
-    KH, E = k_cache.shape[1], k_cache.shape[3]
-    if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, KH, E):
+    shape, dtype = k.shape, k_cache.dtype
+    if len(shape) != 4 or shape != v.shape or shape[0] != B or shape[1] != KH or shape[3] != E:
         raise NNopShapeError(-1, f"{name}: k and v must be (B, KH, T, E) = ({B}, {KH}, T, {E})")
-    if any(t is not None and t.dtype != k_cache.dtype for t in (q, k, v)):
+    if k.dtype is not dtype or v.dtype is not dtype or (q is not None and q.dtype is not dtype):
         raise NNopError(-2, f"{name}: q, k and v must have the dtype of the caches")
-    T = k.shape[2]
+    T = shape[2]
     QH, cb, qo = 0, 1, None
     if cos is not None:
-        cos, sin = _rope_tables(cos, sin, B, T, E)
-        cb = cos.shape[0]
+        cb, f32 = cos.shape[0], torch.float32
+        if cos.shape == (cb, T, E) == sin.shape and cb in (1, B) and cos.dtype is f32 and sin.dtype is f32:
+            cos, sin = cos.contiguous(), sin.contiguous()
+        else:
+            cos, sin = _rope_tables(cos, sin, B, T, E)
+            cb = cos.shape[0]
     if q is not None:
-        if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, T, E):
+        qshape = q.shape
+        if len(qshape) != 4 or qshape[0] != B or qshape[2] != T or qshape[3] != E:
             raise NNopShapeError(-1, f"{name}: q must be (B, QH, T, E) = ({B}, QH, {T}, {E})")
-        QH = q.shape[1]
+        QH = qshape[1]
         q = _aligned(q)
         qo = torch.empty_like(q)
     if n_new is not None:
         if tuple(n_new.shape) != (B,):
             raise NNopShapeError(-1, f"{name}: n_new must be (B,) = ({B},)")
-        if n_new.dtype != torch.int32:
+        if n_new.dtype is not torch.int32:
             raise NNopError(-2, f"{name}: n_new must be int32")
         n_new = n_new.contiguous()
     k, v, lengths, block_table = _aligned(k), _aligned(v), lengths.contiguous(), block_table.contiguous()
     new_lengths = torch.empty_like(lengths)
-    _on(dev, lib.nnop_paged_append, _ptr(q), _ptr(k), _ptr(v), _ptr(cos), _ptr(sin), _ptr(n_new), _ptr(qo),
-        _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(lengths), _ptr(new_lengths), E, T, QH, KH, B, cb, *cache,
-        _dtype_id(k_cache))
+    _on(dev, lib.nnop_paged_append, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos), _ptr(sin), _ptr(n_new), _ptr(qo),
+        k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), new_lengths.data_ptr(), E, T,
+        QH, KH, B, cb, *cache, _dtype_id(k_cache))
     return qo, new_lengths
 
 
@@ -807,29 +828,29 @@ def paged_append_rope(q, k, v, k_cache, v_cache, block_table, lengths, *, cos, s
 def _paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None):
     """``paged_attention`` returning ``(o, lse)``, lse (B, QH, 1) float32."""
     name = "paged_attention"
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (q, weights), False)
+    dev = _paged_device(name, k_cache, v_cache, block_table, lengths, q, weights)
+    B, KH, E, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, False)
     _no_grad(name, q, k_cache, v_cache, weights)
-    KH, E = k_cache.shape[1], k_cache.shape[3]
     shape = q.shape
     if len(shape) != 4 or shape[0] != B or shape[2] != 1:
         raise NNopShapeError(-1, f"{name}: q must be (B, QH, 1, E) with B = {B}")
     if shape[3] != E:
         raise NNopShapeError(-1, f"Embedding dim of Q `{shape[3]}` must be the same as of K `{E}`.")
-    if q.dtype != k_cache.dtype:
+    if q.dtype is not k_cache.dtype:
         raise NNopError(-2, f"{name}: q must have the dtype of the caches")
-    QH = shape[1]
-    if weights is not None:
+    QH, weigh = shape[1], weights is not None
+    if weigh:
         if tuple(weights.shape) != (B, KH, cache[1] * cache[2]):
             raise NNopShapeError(-1, f"{name}: weights must have shape (B, KH, MP·PS) = {(B, KH, cache[1] * cache[2])}")
-        if weights.dtype != torch.float32 or not weights.is_contiguous():
+        if weights.dtype is not torch.float32 or not weights.is_contiguous():
             raise NNopError(-2, f"{name}: weights must be contiguous float32")
-    q, lengths, block_table = _aligned(q), lengths.contiguous(), block_table.contiguous()
-    dt, weigh = _dtype_id(q), weights is not None
-    ws_bytes = lib.nnop_paged_attention_fwd_workspace_size(E, QH, KH, B, cache[1], cache[2], weigh, dt)
+    q, lengths, block_table, dt = _aligned(q), lengths.contiguous(), block_table.contiguous(), _dtype_id(q)
+    ws_bytes = _workspace_bytes(E, QH, KH, B, cache[1], cache[2], weigh, dt)
     o, lse = torch.empty_like(q), q.new_empty((B, QH, 1), dtype=torch.float32)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     _on(dev, lib.nnop_paged_attention_fwd, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-        lengths.data_ptr(), _ptr(weights), o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes, E, QH, KH, B, *cache, dt)
+        lengths.data_ptr(), weights.data_ptr() if weigh else None, o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes,
+        E, QH, KH, B, *cache, dt)
     return o, lse
 
 
@@ -858,9 +879,10 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
     new_weights (B, KH, MP'·PS), kept (B, KH, budget))``: the kept slots' weights
     (0 behind them) and their old slots, ascending (-1 behind them)."""
     name = "paged_evict"
-    dev, B, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, (new_table, weights), True)
+    dev = _paged_device(name, k_cache, v_cache, block_table, lengths, new_table, weights)
+    B, KH, E, cache = _paged_dims(name, k_cache, v_cache, block_table, lengths, True)
+    PS = cache[1]
     _no_grad(name, k_cache, v_cache, weights)
-    P, KH, PS, E = k_cache.shape
     if new_table.dim() != 2 or new_table.shape[0] != B:
         raise NNopShapeError(-1, f"{name}: new_table must be (B, MP') with B = {B}")
     if new_table.dtype != torch.int32:
@@ -876,7 +898,7 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
     block_table, new_table = block_table.contiguous(), new_table.contiguous()
     new_lengths = torch.empty_like(lengths)
     new_weights, kept = weights.new_empty((B, KH, slots)), lengths.new_empty((B, KH, budget))
-    _on(dev, lib.nnop_paged_evict, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(new_table), _ptr(lengths),
-        _ptr(weights), _ptr(new_lengths), _ptr(new_weights), _ptr(kept), E, KH, B, *cache[:3], new_table.shape[1],
-        *cache[3:], budget, recent, _dtype_id(k_cache))
+    _on(dev, lib.nnop_paged_evict, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), new_table.data_ptr(),
+        lengths.data_ptr(), weights.data_ptr(), new_lengths.data_ptr(), new_weights.data_ptr(), kept.data_ptr(), E, KH, B,
+        *cache[:3], new_table.shape[1], *cache[3:], budget, recent, _dtype_id(k_cache))
     return new_lengths, new_weights, kept

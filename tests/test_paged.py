@@ -68,18 +68,67 @@ def test_page_division():
         assert np.array_equal((hi + n) >> np.uint64(s), n // np.uint64(d)), d
 
 
-@pytest.mark.parametrize("ctas", [1, 7, 592])
-def test_split_covers_every_unit_once(ctas):
-    """CTA c of G = min(ctas, U) has units [floor(U·c/G), floor(U·(c+1)/G)), at least
-    one; the CTA of a split's last unit follows from the unit alone."""
-    rng = np.random.default_rng(ctas)
-    for U in [1, 2, 3, ctas + 1, ctas, 10 * ctas + 3, *map(int, rng.integers(1, 5000, 20))]:
-        G = min(ctas, U)
-        start = [U * c // G for c in range(G + 1)]
-        own = [((e + 1) * G + U - 1) // U - 1 for e in range(U)]
-        for c in range(G):
-            assert start[c] < start[c + 1]
-            assert all(own[e] == c for e in range(start[c], start[c + 1]))
+def _segments(lens, heads, ctas, unit, extra, parts):
+    """The kernels' split, restated: for each part its segments (b, h, c0, c1) and, per
+    (b, h), what owner() says of its first and last chunk."""
+    total, some = sum(-(-n // unit) for n in lens), sum(n > 0 for n in lens)
+    extra = extra if total * heads > ctas else 0
+    chunks = [-(-n // unit) + extra if n else 0 for n in lens]
+    units = sum(chunks) * heads
+    G, parts = min(ctas, units), min(parts, units)
+    where = [(b, h, c) for b, n in enumerate(chunks) for h in range(heads) for c in range(n)]
+    segments = []
+    for p in range(parts):
+        u, u1 = units * p // parts, units * (p + 1) // parts
+        mine = []
+        if u < u1:
+            b, h, c0 = where[u]
+            if c0 <= extra:
+                u, c0 = u - c0, 0
+            while u < u1:
+                c1 = min(chunks[b], c0 + u1 - u)
+                if c1 <= extra and c1 < chunks[b]:
+                    break
+                mine.append((b, h, c0, c1))
+                u += c1 - c0
+                if u < u1:
+                    b, h, c0 = where[u]
+                    assert c0 == 0
+        segments.append(mine)
+    first = {bh: i for i, bh in reversed(list(enumerate(w[:2] for w in where)))}
+
+    def owner(e):
+        return ((e + 1) * G + units - 1) // units - 1
+    owners = {(b, h): (owner(u + extra), owner(u + chunks[b] - 1)) for (b, h), u in first.items()}
+    return segments, owners, extra, chunks
+
+
+@pytest.mark.parametrize("ctas", [1, 7, 444])
+@pytest.mark.parametrize("extra", [0, 1, 4, 9])
+def test_split_covers_every_chunk_once(ctas, extra):
+    """Whatever the lengths: every chunk with slots in one part, the parts of a (b, h) in
+    consecutive CTAs from the first to the last that owner() names, so that each CTA has
+    at most one part that begins inside a (b, h) and one that ends inside."""
+    rng = np.random.default_rng(ctas + extra)
+    for trial in range(25):
+        lens = [int(n) for n in rng.integers(0, [1, 3, 40, 700][trial % 4] + 1, rng.integers(1, 12))]
+        heads = int(rng.integers(1, 5))
+        segments, owners, ex, chunks = _segments(lens, heads, ctas, 16, extra, ctas)
+        got = {}
+        for c, mine in enumerate(segments):
+            assert sum(c0 > 0 for _, _, c0, _ in mine) <= 1 and sum(c1 < chunks[b] for b, _, _, c1 in mine) <= 1
+            for b, h, c0, c1 in mine:
+                got.setdefault((b, h), []).append((c, c0, c1))
+        assert set(got) == set(owners) == {(b, h) for b, n in enumerate(lens) if n for h in range(heads)}
+        for (b, h), parts in got.items():
+            assert (parts[0][0], parts[-1][0]) == owners[b, h]
+            assert [p[0] for p in parts] == list(range(parts[0][0], parts[-1][0] + 1))
+            assert parts[0][1] == 0 and parts[-1][2] == chunks[b]
+            assert all(x[2] == y[1] for x, y in zip(parts, parts[1:])) and (len(parts) == 1 or parts[0][2] > ex)
+        # any other number of parts covers the chunks too (the second launch's)
+        seen = [(b, h, c) for mine in _segments(lens, heads, ctas, 16, extra, 3 * ctas + 1)[0]
+                for b, h, c0, c1 in mine for c in range(max(c0, ex), c1)]
+        assert sorted(seen) == [(b, h, c) for b, n in enumerate(chunks) for h in range(heads) for c in range(ex, n)]
 
 
 D = C.c_void_p(4096)      # never dereferenced: every call below is refused before a launch
