@@ -184,20 +184,36 @@ constexpr int kBins = 2048;
 constexpr size_t kHistBytes = sizeof(int) * kDigits * kBins;
 constexpr int kMostKeys = 48 * 1024;                         // of a CTA's share in shared memory
 
+constexpr int kMostCtas = 8;                                 // of a cluster
+
+// Sum over the lanes in front.
+__device__ __forceinline__ int warp_sum_before(int n) {
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if ((threadIdx.x & 31) >= o) incl += up;
+    }
+    return incl - n;
+}
+
 __device__ __forceinline__ int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
 
 // The slots to keep of one (sequence, KV head): a cluster of 1 to 8 CTAs, each with a
 // contiguous share of the slots and its keys in shared memory (read once; a share of
 // more than kMostKeys is read again).  The (budget − recent)-th largest key is found
-// digit by digit: every CTA counts its keys by the digit, sums the cluster's counts
-// through distributed shared memory and walks them from the top.  Then each CTA writes
-// its kept slots in order, behind those of the CTAs in front of it: a slot's place is
-// (larger keys in front) + min(equal keys in front, equals to keep).
+// digit by digit: every CTA counts its keys by the digit and gives every CTA of the
+// cluster its counts of 32 bins at once; one warp of each finds the 32 bins that the
+// wanted key is in, fetches those of the other CTAs through distributed shared memory
+// and finds the bin (all 2048 bins of 8 CTAs, fetched by all threads, take 4 us a digit).
+// Then each CTA writes its kept slots in order, behind those of the CTAs in front of it: a
+// slot's place is (larger keys in front) + min(equal keys in front, equals to keep).
 __global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a, int most_keys) {
-    extern __shared__ int smem[];
+    extern __shared__ __align__(16) int smem[];
     int* hist = smem;                                        // [kDigits][kBins]
     uint32_t* keys = reinterpret_cast<uint32_t*>(smem + kDigits * kBins);
-    __shared__ int pick[2], warp_sum[kSelectWarps], warp_eq[kSelectWarps], mine[2];
+    __shared__ int pick[2], warp_gt[kSelectWarps], warp_eq[kSelectWarps], mine[2];
+    __shared__ __align__(8) int coarse[kDigits][kMostCtas][kBins / 32];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -217,77 +233,116 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a, int 
     const int need = count - last;                                  // of the first `cand`
     for (int i = gt0; i < last; i += all) kept[need + i] = cand + i;
     if (need == 0) return;                                   // the same for the whole cluster
+    auto begun = cluster.barrier_arrive();
     const int share = (cand + C - 1) / C;
     const int i0 = min(rank * share, cand), size = min(share, cand - i0);
     const bool held = size <= most_keys;
     for (int i = t; i < kDigits * kBins; i += kSelectThreads) hist[i] = 0;
     if (held) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = t; i < size; i += kSelectThreads) keys[i] = order_key(w[i0 + i]);
     }
-    __syncthreads();
+    cluster.barrier_wait(std::move(begun));      // every CTA runs: its shared memory may be written
+    __syncthreads();                             // this one's counts are zero, its keys there
+    // Four keys from i (a multiple of 4); 0, which is no number's key, behind the last.
+    auto four = [&](int i) {
+        uint4 k = make_uint4(0, 0, 0, 0);
+        if (held) k = *reinterpret_cast<const uint4*>(keys + i);
+        else {
+            k.x = order_key(w[i0 + i]);
+            if (i + 1 < size) k.y = order_key(w[i0 + i + 1]);
+            if (i + 2 < size) k.z = order_key(w[i0 + i + 2]);
+            if (i + 3 < size) k.w = order_key(w[i0 + i + 3]);
+        }
+        if (i + 1 >= size) k.y = 0;
+        if (i + 2 >= size) k.z = 0;
+        if (i + 3 >= size) k.w = 0;
+        return k;
+    };
     uint32_t prefix = 0;        // digits of the wanted key so far
     int left = need;            // it is the left-th largest of the keys that begin so
+#pragma unroll
     for (int d = 0; d < kDigits; ++d) {
         const int shift = digit_shift(d), above = d == 0 ? 0 : digit_shift(d - 1);
         const int bins = d == 2 ? 1024 : 2048;
         int* h = hist + d * kBins;
-        for (int i = t; i < size; i += kSelectThreads) {
-            const uint32_t key = held ? keys[i] : order_key(w[i0 + i]);
-            if (d == 0 || key >> above == prefix) atomicAdd(&h[(key >> shift) & (bins - 1)], 1);
+        auto add = [&](uint32_t key) {
+            if (key != 0 && (d == 0 || key >> above == prefix)) atomicAdd(&h[(key >> shift) & (bins - 1)], 1);
+        };
+        for (int i = 4 * t; i < size; i += 4 * kSelectThreads) {
+            const uint4 k = four(i);
+            add(k.x);
+            add(k.y);
+            add(k.z);
+            add(k.w);
+        }
+        __syncthreads();
+        // counts of 32 bins: 16 threads with two bins each; lane c of them writes to CTA c
+        if (2 * t < bins) {
+            const int2 two = *reinterpret_cast<const int2*>(h + 2 * t);
+            const int of32 = __reduce_add_sync(lane < 16 ? 0xffffu : 0xffff0000u, two.x + two.y);
+            if ((lane & 15) < C) cluster.map_shared_rank(&coarse[d][rank][t / 16], lane & 15)[0] = of32;
         }
         cluster.sync();
-        // thread t has the t-th pair of bins from the top
-        const int top = bins - 1 - 2 * t;
-        int n1 = 0, n0 = 0;
-        if (top > 0) {
+        if (warp == 0) {
+            // the wanted key's 32 bins, then its bin: lane l has the l-th from the top
+            const int last32 = bins / 32 - 1 - 2 * lane;
+            int n1 = 0, n0 = 0;
+            if (last32 > 0) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c >= C) break;
-                const int2 x = *reinterpret_cast<const int2*>(cluster.map_shared_rank(h, c) + top - 1);
-                n0 += x.x;
-                n1 += x.y;
+                for (int c = 0; c < kMostCtas; ++c) {
+                    if (c >= C) break;
+                    const int2 x = *reinterpret_cast<const int2*>(&coarse[d][c][last32 - 1]);
+                    n0 += x.x;
+                    n1 += x.y;
+                }
             }
-        }
-        int incl = n0 + n1;
+            int over = warp_sum_before(n0 + n1);
+            int in = -1;
+            if (over < left && left <= over + n1) in = last32;
+            else if (over + n1 < left && left <= over + n1 + n0) {
+                in = last32 - 1;
+                over += n1;
+            }
+            const int who = __ffs(__ballot_sync(0xffffffffu, in >= 0)) - 1;
+            in = __shfl_sync(0xffffffffu, in, who);
+            const int rest = left - __shfl_sync(0xffffffffu, over, who);
+            const int bin = in * 32 + 31 - lane;
+            int from[kMostCtas];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += up;
-        }
-        if (lane == 31) warp_sum[warp] = incl;
-        __syncthreads();
-        int over = incl - n0 - n1;      // keys with a larger digit
-        over += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
-        if (over < left && left <= over + n1) {
-            pick[0] = top;
-            pick[1] = left - over;
-        } else if (over + n1 < left && left <= over + n1 + n0) {
-            pick[0] = top - 1;
-            pick[1] = left - over - n1;
+            for (int c = 0; c < kMostCtas; ++c)
+                from[c] = c == rank ? h[bin] : c < C ? cluster.map_shared_rank(h, c)[bin] : 0;
+            int sum = 0;
+#pragma unroll
+            for (int c = 0; c < kMostCtas; ++c) sum += from[c];
+            over = warp_sum_before(sum);
+            if (over < rest && rest <= over + sum) {
+                pick[0] = bin;
+                pick[1] = rest - over;
+            }
         }
         __syncthreads();
         prefix = prefix << (d == 2 ? 10 : 11) | (uint32_t)pick[0];
         left = pick[1];
     }
-    // Larger keys are kept, and the first `left` that equal it.  Each warp has a contiguous run.
-    const int run = ((size + kSelectWarps - 1) / kSelectWarps + 31) & ~31;
-    const int r0 = min(warp * run, size), r1 = min(r0 + run, size);
+    // Larger keys are kept, and the first `left` that equal it.  Each warp has a contiguous
+    // run, each lane four slots of 128.
+    const int run = ((size + kSelectWarps - 1) / kSelectWarps + 127) & ~127;
+    const int r0 = (int)min((int64_t)warp * run, (int64_t)size), r1 = (int)min((int64_t)r0 + run, (int64_t)size);
     int gt = 0, eq = 0;
-    for (int i = r0 + lane; i < r1; i += 32) {
-        const uint32_t key = held ? keys[i] : order_key(w[i0 + i]);
-        gt += key > prefix;
-        eq += key == prefix;
+    for (int i = r0 + 4 * lane; i < r1; i += 128) {
+        const uint4 k = four(i);
+        gt += (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
+        eq += (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
     }
     gt = __reduce_add_sync(0xffffffffu, gt);
     eq = __reduce_add_sync(0xffffffffu, eq);
-    __syncthreads();
     if (lane == 0) {
-        warp_sum[warp] = gt;
+        warp_gt[warp] = gt;
         warp_eq[warp] = eq;
     }
     __syncthreads();
-    const int gt_all = __reduce_add_sync(0xffffffffu, warp_sum[lane]);
+    const int gt_all = __reduce_add_sync(0xffffffffu, warp_gt[lane]);
     const int eq_all = __reduce_add_sync(0xffffffffu, warp_eq[lane]);
     if (t == 0) {
         mine[0] = gt_all;
@@ -295,23 +350,33 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a, int 
     }
     cluster.sync();
     gt = eq = 0;
-    for (int c = 0; c < rank; ++c) {
-        const int* other = cluster.map_shared_rank(mine, c);
-        gt += other[0];
-        eq += other[1];
+    if (lane < rank) {
+        const int* other = cluster.map_shared_rank(mine, lane);
+        gt = other[0];
+        eq = other[1];
     }
-    gt += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
-    eq += __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0);
-    for (int k0 = r0; k0 < r1; k0 += 32) {
-        const int i = k0 + lane;
-        const uint32_t key = i >= r1 ? 0 : held ? keys[i] : order_key(w[i0 + i]);
-        const bool is_gt = i < r1 && key > prefix, is_eq = i < r1 && key == prefix;
-        const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-        const uint32_t before = (1u << lane) - 1;
-        const int g = gt + __popc(mg & before), e = eq + __popc(me & before);
-        if (is_gt || (is_eq && e < left)) kept[g + min(e, left)] = i0 + i;
-        gt += __popc(mg);
-        eq += __popc(me);
+    gt = __reduce_add_sync(0xffffffffu, gt + (lane < warp ? warp_gt[lane] : 0));
+    eq = __reduce_add_sync(0xffffffffu, eq + (lane < warp ? warp_eq[lane] : 0));
+    for (int k0 = r0; k0 < r1; k0 += 128) {
+        const int i = k0 + 4 * lane;
+        const uint4 k = i < r1 ? four(i) : make_uint4(0, 0, 0, 0);
+        const int g4 = (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
+        const int e4 = (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
+        const int both = g4 | e4 << 16, before = warp_sum_before(both);
+        int g = gt + (before & 0xffff), e = eq + (before >> 16);
+        auto put = [&](uint32_t key, int at) {
+            const bool is_eq = key == prefix;
+            if (key > prefix || (is_eq && e < left)) kept[g + min(e, left)] = i0 + at;
+            g += key > prefix;
+            e += is_eq;
+        };
+        put(k.x, i);
+        put(k.y, i + 1);
+        put(k.z, i + 2);
+        put(k.w, i + 3);
+        const int sums = __shfl_sync(0xffffffffu, before + both, 31);
+        gt += sums & 0xffff;
+        eq += sums >> 16;
     }
     cluster.sync();             // no CTA leaves while another may read its shared memory
 }
@@ -363,8 +428,8 @@ __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
 
 int launch_select(const EvictArgs& a, cudaStream_t s) {
     int C = 1;
-    while (C < 8 && a.c.slots / C > 8192 && a.B * a.KH * C * 2 <= num_sms()) C *= 2;
-    const int most_keys = std::min(kMostKeys, (a.c.slots + C - 1) / C);
+    while (C < kMostCtas && a.c.slots / C > 8192 && a.B * a.KH * C * 2 <= num_sms()) C *= 2;
+    const int most_keys = std::min(kMostKeys, ((a.c.slots + C - 1) / C + 3) & ~3);      // whole fours
     const size_t bytes = kHistBytes + sizeof(uint32_t) * (size_t)most_keys;
     if (bytes > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
