@@ -287,32 +287,28 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     }
 }
 
-#ifndef EXTRA
-#define EXTRA 8
-#endif
-#ifndef C1
-#define C1 3
-#endif
-#ifndef C2
-#define C2 2
-#endif
 template <int E> struct MmaShape {
     static constexpr int kTiles = E >= 128 ? 1 : E == 64 ? 2 : 4;   // 16-key tiles a warp takes at once (8 KB of K and V from E = 32)
     static constexpr int kKeys = 16 * kTiles;
     static constexpr int kUnit = kKeys;                             // slots per unit of the split
-    static constexpr int kExtra = EXTRA;
 };
 
 // CTAs per SM.  What has to be in flight to keep HBM busy lies in registers, 8 KB a
 // warp, beside 32·NT for Oᵀ and 16·NT for Q: three CTAs of 168 registers a thread
-// (181 us for 64 sequences up to 8192) before two of 255 (194 us) or four that spill
-// (236 us); with two head tiles a warp, two.
-constexpr int mma_ctas(int E, int NT) { return NT == 1 ? C1 : C2; }
+// (168 us for 64 sequences up to 8192) before two of 255 (174 us) or four that spill
+// (254 us); with two head tiles a warp, two.  A ring in shared memory filled by cp.async,
+// with up to 192 KB in flight, was slower: 173 us, and 107 instead of 90 for heads of 64.
+constexpr int mma_ctas(int NT) { return NT == 1 ? 3 : 2; }
+// What a segment's begin and end count for, in units (8 KB; a CTA among two has a larger
+// share of HBM than one among three).  64 sequences up to 8192: 2 units 172 us, 4 units
+// 168, 8 units 167; 32 of them with two head tiles: 8 units 132 us, 12 units 123, 16 units
+// 110, 24 units 109.
+constexpr int mma_extra(int NT) { return NT == 1 ? 8 : 16; }
 
 // NT: head tiles (of 8) per warp, which share the fragments of K and V.  WT: warps
 // that read the same keys for other head tiles; 4/WT warps share the keys out.
 template <typename T, int E, int NT, int WT, bool kWholeTiles>
-__global__ void __launch_bounds__(kThreads, mma_ctas(E, NT))
+__global__ void __launch_bounds__(kThreads, mma_ctas(NT))
 attention_mma(AttnArgs a) {
     using S = MmaShape<E>;
     constexpr int R = 8 * NT * WT;
@@ -326,7 +322,7 @@ attention_mma(AttnArgs a) {
     const int tile0 = warp % WT * NT, part = warp / WT;
     const int heads = a.KH * a.tiles;
     let_next_start();
-    Split s = split_begin<S::kUnit, S::kExtra>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
+    Split s = split_begin<S::kUnit, mma_extra(NT)>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
     write_empty<T, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     int c1 = s.segment();
@@ -339,16 +335,17 @@ attention_mma(AttnArgs a) {
     const char *kl, *vl;           // this head's pools, at this lane's first row and bytes of a tile
     // Bytes between a lane's rows: K 8 rows on; V 1, 8 and 9 rows on.
     const int64_t rs = a.c.row_stride * 2;
+    const bool odd_pages = a.c.page_size.d & 1;
     constexpr int kStep = S::kKeys * (4 / WT);
 
     // Where a step's rows are.  kWholeTiles (pages of a multiple of 16 slots): a tile of 16
-    // keys lies in one page, one lookup for all lanes, made a step ahead (168 us for 64
-    // sequences up to 8192; 175 when it is made with the loads).  Else one lookup for each
-    // row a lane reads (pages of 20: 191 us; a step ahead in other lanes and handed out by
-    // shuffles: 221).
+    // keys lies in one page, one lookup for all lanes, its table entry fetched a step ahead
+    // (168 us for 64 sequences up to 8192; 175 when it is fetched with the rows).  Else one
+    // lookup for each row a lane reads (pages of 20: 169 us, but heads of 64 in pages of 16
+    // would take 107 us that way instead of 90, heads of 32 93 instead of 54).
     uint32_t page[S::kTiles];      // table entries of the next step's tiles
     int row[S::kTiles];
-    int64_t tiles[S::kTiles];      // bytes into the pool; negative: no page
+    int64_t tiles[S::kTiles] = {}; // bytes into the pool; negative: no page
     bool inside;                   // all of the step's keys have rows
     auto find = [&](int key0) {
         if constexpr (kWholeTiles) {
@@ -374,50 +371,51 @@ attention_mma(AttnArgs a) {
         const int64_t x = a.c.offset(tab, key + mine);
         return x < 0 ? -1 : x * 2;
     };
-    // K of the step at key0; bit 2t + i: this lane's key 16t + 8i + gid has a row.
-    auto load_k = [&](int key0) -> uint32_t {
-        if (inside) {
+    // Where a lane reads K of tile t, rows gid and 8 + gid; bit 2t + i of has: there is a row.
+    auto k_rows = [&](const char* (&p)[2], int t, int key0, uint32_t& has) {
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], kl + tiles[t] + i * 8 * rs + c * (16 * KW));
-            return ~0u;
+        for (int i = 0; i < 2; ++i) {
+            const int64_t x = row_at(t, key0 + t * 16, i * 8 + gid, gid);
+            if (x < 0) has &= ~(1u << (2 * t + i));
+            p[i] = x >= 0 ? kl + x : reinterpret_cast<const char*>(no_row);
         }
-        uint32_t has = 0;
+    };
+    // ... and V of tile t, rows 2·sub, 2·sub + 1 and both 8 on.
+    auto v_rows = [&](const char* (&p)[4], int t, int key0) {
+        int64_t x = -1;
 #pragma unroll
-        for (int t = 0; t < S::kTiles; ++t)
+        for (int i = 0; i < 4; ++i) {
+            const int mine = (i >> 1) * 8 + (i & 1) + 2 * sub;
+            // pages of an even number of slots hold both keys of a pair
+            if (kWholeTiles || i % 2 == 0 || odd_pages) x = row_at(t, key0 + t * 16, mine, 2 * sub);
+            else x = x < 0 || key0 + t * 16 + mine >= end ? -1 : x + rs;
+            p[i] = x >= 0 ? vl + x : reinterpret_cast<const char*>(no_row);
+        }
+    };
+    auto load_k = [&](int key0, uint32_t& has) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t x = row_at(t, key0 + t * 16, i * 8 + gid, gid);
-                has |= (uint32_t)(x >= 0) << (2 * t + i);
-                const char* p = x >= 0 ? kl + x : reinterpret_cast<const char*>(no_row);
+        for (int t = 0; t < S::kTiles; ++t) {
+            const char* p[2] = {};
+            if (!inside) k_rows(p, t, key0, has);
 #pragma unroll
-                for (int c = 0; c < KC; ++c) load_words<KW>(kr[t][i][c], p + c * (16 * KW));
-            }
-        return has;
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+                    load_words<KW>(kr[t][i][c], (inside ? kl + tiles[t] + i * 8 * rs : p[i]) + c * (16 * KW));
+        }
     };
     auto load_v = [&](int key0) {
-        if (inside) {
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t)
+        for (int t = 0; t < S::kTiles; ++t) {
+            const char* p[4] = {};
+            if (!inside) v_rows(p, t, key0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int c = 0; c < VC; ++c)
-                        load_words<VW>(vr[t][i][c], vl + tiles[t] + ((i >> 1) * 8 + (i & 1)) * rs + c * (32 * VW));
-            return;
+                for (int c = 0; c < VC; ++c)
+                    load_words<VW>(vr[t][i][c],
+                                   (inside ? vl + tiles[t] + ((i >> 1) * 8 + (i & 1)) * rs : p[i]) + c * (32 * VW));
         }
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t x = row_at(t, key0 + t * 16, (i >> 1) * 8 + (i & 1) + 2 * sub, 2 * sub);
-                const char* p = x >= 0 ? vl + x : reinterpret_cast<const char*>(no_row);
-#pragma unroll
-                for (int c = 0; c < VC; ++c) load_words<VW>(vr[t][i][c], p + c * (32 * VW));
-            }
     };
     uint32_t live = 0;
     // The segment [s.chunk, c1) of (s.b, s.h): its Q, and the first step's K and V.
@@ -441,7 +439,8 @@ attention_mma(AttnArgs a) {
         }
         if (key0 < end) {
             found(key0);
-            live = load_k(key0);
+            live = ~0u;
+            load_k(key0, live);
             load_v(key0);
             find(key0 + kStep);
         }
@@ -466,26 +465,35 @@ attention_mma(AttnArgs a) {
                     for (int i = 0; i < 4; ++i) acc[n][c][j][i] = 0.f;
         }
         for (; key0 < end; key0 += kStep) {
+            // Pages of other sizes: each chunk's registers are loaded again as soon as its
+            // products are through (pages of 20: 169 us instead of 179).
+            const bool more = key0 + kStep < end;
+            uint32_t next = ~0u;
+            if (more) found(key0 + kStep);
             float d[NT][S::kTiles][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int t = 0; t < S::kTiles; ++t) {
+                const char* p[2] = {};
+                if (!kWholeTiles && more) k_rows(p, t, key0 + kStep, next);
 #pragma unroll
-                for (int t = 0; t < S::kTiles; ++t) {
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) d[n][t][i] = 0.f;
 #pragma unroll
-                    for (int c = 0; c < KC; ++c)
+                for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int w = 0; w < KW; w += 2)
                             mma16816<T>(d[n][t], kr[t][0][c][w], kr[t][1][c][w], kr[t][0][c][w + 1], kr[t][1][c][w + 1],
                                         q[n][c][w], q[n][c][w + 1]);
+                    if (!kWholeTiles && more) {
+                        load_words<KW>(kr[t][0][c], p[0] + c * (16 * KW));
+                        load_words<KW>(kr[t][1][c], p[1] + c * (16 * KW));
+                    }
                 }
-            const bool more = key0 + kStep < end;
-            uint32_t next = 0;
-            if (more) {
-                found(key0 + kStep);
-                next = load_k(key0 + kStep);
             }
+            if (kWholeTiles && more) load_k(key0 + kStep, next);
             if (live != ~0u) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -551,9 +559,11 @@ attention_mma(AttnArgs a) {
                     }
             }
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t)
+            for (int t = 0; t < S::kTiles; ++t) {
+                const char* p[4] = {};
+                if (!kWholeTiles && more) v_rows(p, t, key0 + kStep);
 #pragma unroll
-                for (int c = 0; c < VC; ++c)
+                for (int c = 0; c < VC; ++c) {
 #pragma unroll
                     for (int j = 0; j < VW; ++j) {
                         const uint32_t a0 = __byte_perm(vr[t][0][c][j], vr[t][1][c][j], 0x5410);
@@ -566,7 +576,13 @@ attention_mma(AttnArgs a) {
                             mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][1][0], b[n][t][1][1]);
                         }
                     }
-            if (more) load_v(key0 + kStep);
+                    if (!kWholeTiles && more) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) load_words<VW>(vr[t][i][c], p[i] + c * (32 * VW));
+                    }
+                }
+            }
+            if (kWholeTiles && more) load_v(key0 + kStep);
             live = next;
             find(key0 + 2 * kStep);
         }
@@ -657,7 +673,7 @@ __device__ __forceinline__ float join_lse2(const float2* part_ml, int R, int c, 
 // group of exp(s_j − lse) for a share of the slots; a split row's lse comes from its
 // parts again, so that both run at once.
 template <typename T, int E, int R, int kUnit, int kExtra>
-__global__ void __launch_bounds__(kThreads) attention_join(AttnArgs a, int rows, int ctas, int adders) {
+__global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int rows, int ctas, int adders) {
     constexpr int LE = E / 4;                             // lanes per row of 16-byte vectors
     constexpr int NP = kThreads / LE;                     // parts at once
     __shared__ __align__(16) union {
@@ -667,6 +683,7 @@ __global__ void __launch_bounds__(kThreads) attention_join(AttnArgs a, int rows,
         } j;
         struct {
             SplitShared split;
+            int first[32], last[32];      // CTAs with the parts of a query head
             float lse2[32];
         } w;
     } sh;
@@ -705,10 +722,11 @@ __global__ void __launch_bounds__(kThreads) attention_join(AttnArgs a, int rows,
         }
         return;
     }
-    // The first launch's split again, which rests on the call's arguments alone.
+    // The first launch's split again, which rests on the call's arguments alone, as do the
+    // weights so far: all of it goes ahead of the wait for the first launch.
     const int heads = a.KH * a.tiles;
     Split s = split_begin<kUnit, kExtra>(a.c, a.B, heads, ctas, blockIdx.x, adders, sh.w.split);
-    wait_before();
+    bool waited = false;
     while (const int c1 = s.segment()) {
         const int end = s.end_slot<kUnit>(c1);
         const int kvh = s.h / a.tiles;
@@ -719,33 +737,41 @@ __global__ void __launch_bounds__(kThreads) attention_join(AttnArgs a, int rows,
             for (int g0 = 0; g0 < a.group; g0 += 32) {
                 const int n = min(32, a.group - g0);
                 __syncthreads();
-                for (int g = t / 32; g < n; g += kThreads / 32) {
-                    const int tile = (g0 + g) / R, r = (g0 + g) % R;
+                if (t < n) {
                     // head tile h of sequence b has units before·heads + h·chunks + [0, chunks)
-                    const long long u = s.before * heads + (long long)(s.h + tile) * s.chunks;
-                    const int first = s.owner(u + s.extra), last = s.owner(u + s.chunks - 1);
-                    const float lse2 = first == last ? a.lse[row0 + g0 + g] * kLog2e
-                                                     : join_lse2(a.part_ml, R, first, last - first + 1, r);
-                    if (t % 32 == 0) sh.w.lse2[g] = lse2;
+                    const long long u = s.before * heads + (long long)(s.h + (g0 + t) / R) * s.chunks;
+                    sh.w.first[t] = s.owner(u + s.extra);
+                    sh.w.last[t] = s.owner(u + s.chunks - 1);
                 }
-                __syncthreads();
                 // four slots a thread at once: their loads do not wait for one another
-                for (int j0 = s.first_slot<kUnit>(s.chunk) + t; j0 < end; j0 += 4 * kThreads) {
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int j0 = s.first_slot<kUnit>(s.chunk) + t; j0 - t < end; j0 += 4 * kThreads) {
+                    float sum[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = j0 + i * kThreads < end ? w[j0 + i * kThreads] : 0.f;
+                    if (j0 - t == s.first_slot<kUnit>(s.chunk)) {
+                        if (!waited) wait_before();
+                        waited = true;
+                        __syncthreads();
+                        for (int g = t / 32; g < n; g += kThreads / 32) {
+                            const int first = sh.w.first[g], parts = sh.w.last[g] - first + 1;
+                            const float lse2 = parts == 1 ? a.lse[row0 + g0 + g] * kLog2e
+                                                          : join_lse2(a.part_ml, R, first, parts, (g0 + g) % R);
+                            if (t % 32 == 0) sh.w.lse2[g] = lse2;
+                        }
+                        __syncthreads();
+                    }
+                    float add[4] = {0.f, 0.f, 0.f, 0.f};
                     for (int g = 0; g < n; ++g) {
                         const float lse2 = sh.w.lse2[g];
                         const float* sc = a.scores + (row0 + g0 + g) * a.c.slots;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int j = j0 + i * kThreads;
-                            if (j < end && lse2 != -INFINITY) sum[i] += fast_exp2(sc[j] - lse2);
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            if (j0 + i * kThreads < end && lse2 != -INFINITY)
+                                add[i] += fast_exp2(sc[j0 + i * kThreads] - lse2);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = j0 + i * kThreads;
-                        if (j < end) w[j] += sum[i];
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (j0 + i * kThreads < end) w[j0 + i * kThreads] = sum[i] + add[i];
                 }
             }
         }
@@ -793,7 +819,7 @@ int launch(const AttnArgs& a, cudaStream_t s) {
         attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
     } else {
         constexpr int NT = R == 8 ? 1 : 2, WT = R / (8 * NT);
-        G = std::min(kMaxCtas, mma_ctas(E, NT) * num_sms());
+        G = std::min(kMaxCtas, mma_ctas(NT) * num_sms());
         if (a.c.page_size.d % 16 == 0)
             attention_mma<T, E, NT, WT, true><<<G, kThreads, 0, s>>>(a);
         else
@@ -802,7 +828,7 @@ int launch(const AttnArgs& a, cudaStream_t s) {
     if (const int rc = check_launch("paged_attention")) return rc;
     const int rows = std::min(R, a.group), adders = a.weights != nullptr ? 8 * num_sms() : 0;
     return launch_dependent("paged_attention",
-                            attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit, f32 ? kExtra : MmaShape<E>::kExtra>,
+                            attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit, f32 ? kExtra : mma_extra(R == 8 ? 1 : 2)>,
                             dim3(adders + G * rows), dim3(kThreads), 0, s, a, rows, G, adders);
 }
 
