@@ -427,12 +427,18 @@ __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
 }
 
 int launch_select(const EvictArgs& a, cudaStream_t s) {
+    // More CTAs for a row while each has over 8192 slots and the GPU has SMs for them: one
+    // sequence of 131067 (8 rows) takes 133, 82, 39 and 33 us with 1, 2, 4 and 8, but 16 of up
+    // to 8192 (128 rows) 60, 62, 72 and 97.
     int C = 1;
     while (C < kMostCtas && a.c.slots / C > 8192 && a.B * a.KH * C * 2 <= num_sms()) C *= 2;
     const int most_keys = std::min(kMostKeys, ((a.c.slots + C - 1) / C + 3) & ~3);      // whole fours
     const size_t bytes = kHistBytes + sizeof(uint32_t) * (size_t)most_keys;
-    if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    // 48 KB, the kernel's own arrays included, need no leave; what is set is the most it can
+    // ask for, so that calls of several threads do not take it from one another
+    if (bytes > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)(kHistBytes + sizeof(uint32_t) * kMostKeys));
         if (e != cudaSuccess) {
             cudaGetLastError();
             return fail(NNOP_ERR_CUDA, std::string("paged_evict: ") + cudaGetErrorString(e));

@@ -473,10 +473,106 @@ def test_evict_types_and_pages(dtype, E, PS):
     check_evict(c, w, 30, 4)
 
 
-@pytest.mark.parametrize("kind", ["spread", "ties"])
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal", "special"])
 def test_evict_long(kind):
+    """Rows whose slots a cluster of CTAs shares, the second much shorter than its table."""
     c = Cache(31, "f16", 2, 16, 64, [70001, 33333], spare=400, clean=True)
     check_evict(c, _weights(c, kind), 9001, 100)
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_evict_rows_larger_than_shared_memory(kind):
+    """Many rows leave a CTA each; a share that does not fit its shared memory is read again
+    in every pass.  All sequences share their pages."""
+    import torch
+
+    import nnop
+    rng = np.random.default_rng(33)
+    B, KH, E, PS, MP, budget = 40, 2, 16, 64, 900, 5000
+    cols = -(-budget // PS)
+    P = MP + B * cols
+    kc, vc = (to_dev(rng.standard_normal((P, KH, PS, E)), "f16") for _ in range(2))
+    table = np.repeat(np.arange(MP, dtype=np.int32)[None], B, 0)
+    new_table = (MP + np.arange(B * cols, dtype=np.int32)).reshape(B, cols)
+    lengths = np.array([57600, 49157, 49152] + [7] * (B - 3), np.int32)
+    w = np.exp(rng.standard_normal((B, KH, MP * PS))) if kind == "spread" else rng.integers(0, 3, (B, KH, MP * PS))
+    w = w.astype(np.float32)
+    want = orc.paged_evict(to_np(kc), to_np(vc), table, new_table, lengths, w, budget=budget, recent=11)
+    got = nnop.paged_evict(kc, vc, *(torch.from_numpy(x).cuda() for x in (table, new_table, lengths, w)), budget=budget,
+                           recent=11)
+    assert np.array_equal(got[2].cpu().numpy(), want[4]) and np.array_equal(got[1].cpu().numpy(), want[3])
+    assert np.array_equal(to_np(kc), want[0]) and np.array_equal(to_np(vc), want[1])
+
+
+def test_captured_eviction():
+    """A captured eviction replays with the weights and lengths that the device holds then."""
+    import torch
+
+    import nnop
+    c = Cache(34, "bf16", 2, 32, 16, [40000, 900], spare=2 * 20, clean=True)
+    free = np.setdiff1d(np.arange(c.P), c.table)[:40].reshape(2, 20).astype(np.int32)
+    new_table, w = torch.from_numpy(free).cuda(), torch.rand(2, 2, c.MP * 16, device="cuda")
+    call = lambda: nnop.paged_evict(c.k, c.v, c.t, new_table, c.n, w, budget=300, recent=20)  # noqa: E731
+    call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for n in ([40000, 900], [12, 300], [0, 31234]):
+        c.lengths = np.array(n, np.int32)
+        c.n.copy_(torch.from_numpy(c.lengths))
+        w.copy_(torch.rand_like(w))
+        want = orc.paged_evict(*c.np()[:3], free, c.lengths, w.cpu().numpy(), budget=300, recent=20)
+        g.replay()
+        assert np.array_equal(out[2].cpu().numpy(), want[4]) and np.array_equal(out[0].cpu().numpy(), want[2])
+        assert np.array_equal(out[1].cpu().numpy(), want[3]) and np.array_equal(to_np(c.v), want[1])
+
+
+def test_evict_at_every_size_of_shared_memory():
+    """Tables whose keys ask for shared memory from below to above what needs leave, each in
+    a process of its own: leave that an earlier call got must not hide one that is missing."""
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path.insert(0, {path!r})
+import nnop
+MP = int(sys.argv[1])
+i32 = dict(device='cuda', dtype=torch.int32)
+k = torch.zeros(MP + 1, 1, 16, 16, device='cuda')
+t = torch.arange(MP, **i32)[None]
+w = torch.arange(MP * 16, device='cuda', dtype=torch.float32).view(1, 1, -1)
+_, _, kept = nnop.paged_evict(k, k.clone(), t, torch.tensor([[MP]], **i32), torch.tensor([MP * 16], **i32), w, budget=16)
+assert kept.flatten().tolist() == list(range(MP * 16 - 16, MP * 16))
+"""
+    import pathlib
+    path = str(pathlib.Path(__file__).resolve().parent.parent / "onionop.jl_b200")
+    runs = [subprocess.Popen([sys.executable, "-c", code.format(path=path), str(mp)], stderr=subprocess.PIPE, text=True)
+            for mp in (100, 200, 320, 400, 512, 1900, 2500, 4000)]
+    for r in runs:
+        _, err = r.communicate(timeout=300)
+        assert r.returncode == 0, err[-1000:]
+
+
+def test_evictions_side_by_side():
+    """Two streams evict different sequences of one pool at once."""
+    import torch
+
+    import nnop
+    c = Cache(35, "f16", 4, 64, 16, [9000, 3000], spare=2 * 30, clean=True)
+    free = np.setdiff1d(np.arange(c.P), c.table)[:60].reshape(2, 30).astype(np.int32)
+    w = c.rng.random((2, 4, c.MP * 16)).astype(np.float32)
+    want = orc.paged_evict(*c.np()[:3], free, c.lengths, w, budget=480, recent=7)
+    new_table, wd = torch.from_numpy(free).cuda(), torch.from_numpy(w).cuda()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for b, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(nnop.paged_evict(c.k, c.v, c.t[b:b + 1], new_table[b:b + 1], c.n[b:b + 1], wd[b:b + 1], budget=480,
+                                        recent=7))
+    torch.cuda.synchronize()
+    for i, k in ((0, 2), (1, 3), (2, 4)):
+        assert np.array_equal(torch.cat([x[i] for x in got]).cpu().numpy(), want[k])
+    assert np.array_equal(to_np(c.k), want[0]) and np.array_equal(to_np(c.v), want[1])
 
 
 def test_evict_keeps_shared_pages_and_drops_what_has_no_page():

@@ -187,6 +187,7 @@ def test_attention_refusals():
     need = lib.nnop_paged_attention_fwd_workspace_size(64, 4, 2, 1, 16, 2, 0, 2)
     assert need > 0 and _attend(lib, nbytes=need - 1) == -4
     assert _attend(lib, ws=C.c_void_p(4096 + 16)) == -6 and _attend(lib, q=C.c_void_p(8)) == -6
+    assert _attend(lib, B=65535, QH=65534, KH=2, PS=1 << 20, MP=1 << 10) == -1      # 2^62 scores
     # with weights the workspace also holds a score per query head and slot
     assert lib.nnop_paged_attention_fwd_workspace_size(64, 4, 2, 1, 16, 2, 1, 2) >= need + 4 * 32 * 4
 
