@@ -24,9 +24,7 @@ namespace nnop {
 namespace paged {
 namespace {
 
-constexpr int kUnit = 64;          // slots per unit: 16 per warp
-constexpr int kExtra = 1;
-constexpr int kMaxCtas = 592;      // 148 SMs × 4; the workspace is sized for it
+constexpr int kMaxCtas = 444;      // 148 SMs × 3; the workspace is sized for it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -67,24 +65,34 @@ __device__ __forceinline__ void write_empty(const AttnArgs& a) {
     }
 }
 
-// CUDA-core kernel: a quad of lanes per key for the scores, E/32 columns per lane
-// for the products with V; R query heads per pass over the keys.
-template <typename T, int E, int R>
-__global__ void __launch_bounds__(kThreads)
+// What stands for a row that is not there: a finite V, so that its weight of 0 counts.
+__device__ const uint4 no_row[16] = {};
+
+template <int E> struct SimtShape {
+    static constexpr int kGroups = E >= 128 ? 1 : E == 64 ? 2 : 4;   // of 8 keys that a warp takes at once (8 KB of K and V from E = 32)
+    static constexpr int kUnit = 8 * kGroups;                        // slots per unit of the split
+};
+constexpr int kSimtExtra = 8;      // units that a segment's begin and end cost (as in attention_mma)
+
+// fp32 (no tensor cores: their formats would cost its accuracy): a quad of lanes per key
+// for the scores, E/32 columns per lane for the products with V, R query heads per pass
+// over the keys.  A step's rows are all in flight before any is used, K of the next step
+// while this one's softmax runs, V while the next scores do: loads under a branch, one
+// at a time, took 259 us where this takes 104 (16 sequences up to 8192, 32/8 heads of 128).
+template <int E, int R>
+__global__ void __launch_bounds__(kThreads, 3)
 attention_simt(AttnArgs a) {
-    constexpr int VEC = 16 / sizeof(T);
-    constexpr int NV = E / VEC;                       // 16-byte vectors per row
-    constexpr int NQ = (NV + 3) / 4;                  // ... per lane of a quad
+    constexpr int NQ = E >= 16 ? E / 16 : 1;          // 16-byte vectors per lane of a quad
     constexpr int COLS = E >= 32 ? E / 32 : 1;        // columns per lane
-    constexpr int kKeys = kUnit / 4;                  // keys per warp and unit
+    constexpr int KG = SimtShape<E>::kGroups, kKeys = 8 * KG, kUnit = SimtShape<E>::kUnit;
     __shared__ SplitShared sh;
     __shared__ __align__(16) float qs[R][E];
     __shared__ float wm[4][R], wl[4][R], wacc[4][R][E];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, sub = lane & 3;
     const int heads = a.KH * a.tiles;
     let_next_start();
-    Split s = split_begin<kUnit, kExtra>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
-    write_empty<T, E>(a);
+    Split s = split_begin<kUnit, kSimtExtra>(a.c, a.B, heads, gridDim.x, blockIdx.x, gridDim.x, sh);
+    write_empty<float, E>(a);
     if (threadIdx.x == 0) a.join[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (const int c1 = s.segment()) {
         const int c0 = s.chunk;
@@ -92,11 +100,11 @@ attention_simt(AttnArgs a) {
         const int rows = min(R, a.group - r0);
         const int qh0 = kvh * a.group + r0;
         const int* tab = a.c.table + (int64_t)s.b * a.c.max_pages;
-        const int64_t ho = (int64_t)kvh * a.c.head_stride;
-        const T* K = static_cast<const T*>(a.k);
-        const T* V = static_cast<const T*>(a.v);
+        const float* K = static_cast<const float*>(a.k) + kvh * a.c.head_stride;
+        const float* V = static_cast<const float*>(a.v) + kvh * a.c.head_stride;
+        const float* none = reinterpret_cast<const float*>(no_row);
         for (int i = threadIdx.x; i < R * E; i += kThreads)
-            qs[i / E][i % E] = i / E < rows ? to_f(static_cast<const T*>(a.q)[((int64_t)s.b * a.QH + qh0) * E + i]) : 0.f;
+            qs[i / E][i % E] = i / E < rows ? static_cast<const float*>(a.q)[((int64_t)s.b * a.QH + qh0) * E + i] : 0.f;
         __syncthreads();
         float m[R], l[R], acc[R][COLS];
 #pragma unroll
@@ -107,95 +115,131 @@ attention_simt(AttnArgs a) {
             for (int i = 0; i < COLS; ++i) acc[r][i] = 0.f;
         }
         const int end = s.end_slot<kUnit>(c1);
-        for (int key0 = s.first_slot<kUnit>(c0) + warp * kKeys; key0 < end; key0 += kUnit) {
-            int64_t off[kKeys / 8];
-            float sc[kKeys / 8][R];
+        constexpr int kStep = 4 * kKeys;
+        float4 kr[KG][NQ];
+        float vr[KG][8][COLS];
+        int64_t off[KG];               // of this quad's keys; negative: no row
+        auto load_k = [&](int64_t (&o)[KG], int key0) {
 #pragma unroll
-            for (int p = 0; p < kKeys / 8; ++p) {
-                const int key = key0 + p * 8 + quad;
-                off[p] = key < end ? a.c.offset(tab, key) : -1;
-                float dot[R];
+            for (int g = 0; g < KG; ++g) {
+                const int key = key0 + g * 8 + quad;
+                o[g] = key < end ? a.c.offset(tab, key) : -1;
+                const float* p = o[g] >= 0 ? K + o[g] + sub * 4 : none;
 #pragma unroll
-                for (int r = 0; r < R; ++r) dot[r] = 0.f;
+                for (int i = 0; i < NQ; ++i) kr[g][i] = __ldcs(reinterpret_cast<const float4*>(p + (o[g] >= 0 ? i * 16 : 0)));
+            }
+        };
+        auto load_v = [&](const int64_t (&o)[KG]) {
 #pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    const int vi = i * 4 + sub;
-                    if (off[p] >= 0 && (NV % 4 == 0 || vi < NV)) {
-                        float kv[VEC];
-                        load_vec<T, VEC>(kv, K + ho + off[p] + vi * VEC);
+            for (int g = 0; g < KG; ++g)
 #pragma unroll
-                        for (int r = 0; r < R; ++r)
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e) dot[r] = fmaf(kv[e], qs[r][vi * VEC + e], dot[r]);
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t x = __shfl_sync(0xffffffffu, o[g], j * 4);
+                    const float* p = x >= 0 && lane * COLS < E ? V + x + lane * COLS : none;
+                    load_vec<float, COLS>(vr[g][j], p);
                 }
+        };
+        int key0 = s.first_slot<kUnit>(c0) + warp * kKeys;
+        if (key0 < end) {
+            load_k(off, key0);
+            load_v(off);
+        }
+        for (; key0 < end; key0 += kStep) {
+            float sc[KG][R];
+#pragma unroll
+            for (int g = 0; g < KG; ++g)
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 1);
-                    dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], 2);
-                    sc[p][r] = off[p] >= 0 ? dot[r] * a.scale2 : -INFINITY;
-                    if (a.scores != nullptr && key < end && sub == 0 && r < rows)
-                        a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = sc[p][r];
+                    float dot = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        const float4 x = *reinterpret_cast<const float4*>(&qs[r][(i * 4 + sub) * 4]);
+                        dot = fmaf(kr[g][i].x, x.x, dot);
+                        dot = fmaf(kr[g][i].y, x.y, dot);
+                        dot = fmaf(kr[g][i].z, x.z, dot);
+                        dot = fmaf(kr[g][i].w, x.w, dot);
+                    }
+                    sc[g][r] = dot;
                 }
+            const bool more = key0 + kStep < end;
+            int64_t here[KG];
+#pragma unroll
+            for (int g = 0; g < KG; ++g) here[g] = off[g];
+            if (more) load_k(off, key0 + kStep);
+#pragma unroll
+            for (int g = 0; g < KG; ++g)
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float x = sc[g][r];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    sc[g][r] = here[g] >= 0 ? x * a.scale2 : -INFINITY;
+                }
+            if (a.scores != nullptr && sub == 0) {
+#pragma unroll
+                for (int g = 0; g < KG; ++g)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const int key = key0 + g * 8 + quad;
+                        if (key < end && r < rows)
+                            a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = sc[g][r];
+                    }
             }
-            float p[kKeys / 8][R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float mx = m[r];
+                float mx = sc[0][r];
 #pragma unroll
-                for (int i = 0; i < kKeys / 8; ++i) mx = fmaxf(mx, sc[i][r]);
+                for (int g = 1; g < KG; ++g) mx = fmaxf(mx, sc[g][r]);
+                // the maximum rises only now and then: the lanes meet only when one of them has more
+                if (__any_sync(0xffffffffu, mx > m[r])) {
+                    mx = fmaxf(mx, m[r]);
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float base = mx == -INFINITY ? 0.f : mx;      // no score yet
-                const float alpha = fast_exp2(m[r] - base);
-                m[r] = mx;
-                float sum = 0.f;
+                    for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    const float alpha = fast_exp2(m[r] - mx);
+                    m[r] = mx;
+                    l[r] *= alpha;
 #pragma unroll
-                for (int i = 0; i < kKeys / 8; ++i) {
-                    p[i][r] = fast_exp2(sc[i][r] - base);
-                    sum += p[i][r];
+                    for (int i = 0; i < COLS; ++i) acc[r][i] *= alpha;
                 }
+                const float base = m[r] == -INFINITY ? 0.f : m[r];      // no score yet
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                l[r] = l[r] * alpha + sum;
-#pragma unroll
-                for (int i = 0; i < COLS; ++i) acc[r][i] *= alpha;
-            }
-#pragma unroll
-            for (int j = 0; j < kKeys; ++j) {
-                const int64_t vo = __shfl_sync(0xffffffffu, off[j / 8], (j % 8) * 4);
-                float vv[COLS];
-#pragma unroll
-                for (int i = 0; i < COLS; ++i) vv[i] = 0.f;
-                if (vo >= 0 && lane * COLS < E) load_vec<T, COLS>(vv, V + ho + vo + lane * COLS);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float pj = __shfl_sync(0xffffffffu, p[j / 8][r], (j % 8) * 4);
-#pragma unroll
-                    for (int i = 0; i < COLS; ++i) acc[r][i] = fmaf(pj, vv[i], acc[r][i]);
+                for (int g = 0; g < KG; ++g) {
+                    sc[g][r] = fast_exp2(sc[g][r] - base);
+                    l[r] += sc[g][r];
                 }
             }
+#pragma unroll
+            for (int g = 0; g < KG; ++g)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float p = __shfl_sync(0xffffffffu, sc[g][r], j * 4);
+#pragma unroll
+                        for (int i = 0; i < COLS; ++i) acc[r][i] = fmaf(p, vr[g][j][i], acc[r][i]);
+                    }
+            if (more) load_v(off);
         }
         // join the warps
-        if (lane == 0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+            if (lane == 0) {
                 wm[warp][r] = m[r];
                 wl[warp][r] = l[r];
             }
-        }
-        if (lane * COLS < E) {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
+            if (lane * COLS < E) {
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) wacc[warp][r][lane * COLS + i] = acc[r][i];
+            }
         }
         __syncthreads();
         const bool whole = c0 == 0 && c1 == s.chunks;
         const int slot = 2 * blockIdx.x + (c0 == 0 ? 1 : 0);
         for (int i = threadIdx.x; i < rows * E; i += kThreads) {
             const int r = i / E, e = i % E;
-            float mx = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+            const float mx = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
             const float base = mx == -INFINITY ? 0.f : mx;
             float sum = 0.f, ac = 0.f;
 #pragma unroll
@@ -205,7 +249,7 @@ attention_simt(AttnArgs a) {
                 ac = fmaf(wacc[w][r][e], f, ac);
             }
             if (whole) {
-                write_row<T, E>(a, s.b, qh0 + r, e, ac, mx, sum);
+                write_row<float, E>(a, s.b, qh0 + r, e, ac, mx, sum);
             } else {
                 a.part_acc[((int64_t)slot * R + r) * E + e] = ac;
                 if (e == 0) a.part_ml[slot * R + r] = make_float2(mx, sum);
@@ -263,9 +307,6 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[W], const char* p) {
     else
         asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(p));
 }
-
-// What stands for a row that is not there: a finite V, so that its weight of 0 counts.
-__device__ const uint4 no_row[16] = {};
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -815,8 +856,8 @@ int launch(const AttnArgs& a, cudaStream_t s) {
     int G;
     constexpr bool f32 = std::is_same<T, float>::value;
     if constexpr (f32) {
-        G = std::min(kMaxCtas, 4 * num_sms());
-        attention_simt<T, E, R><<<G, kThreads, 0, s>>>(a);
+        G = std::min(kMaxCtas, 3 * num_sms());
+        attention_simt<E, R><<<G, kThreads, 0, s>>>(a);
     } else {
         constexpr int NT = R == 8 ? 1 : 2, WT = R / (8 * NT);
         G = std::min(kMaxCtas, mma_ctas(NT) * num_sms());
@@ -828,7 +869,8 @@ int launch(const AttnArgs& a, cudaStream_t s) {
     if (const int rc = check_launch("paged_attention")) return rc;
     const int rows = std::min(R, a.group), adders = a.weights != nullptr ? 8 * num_sms() : 0;
     return launch_dependent("paged_attention",
-                            attention_join<T, E, R, f32 ? kUnit : MmaShape<E>::kUnit, f32 ? kExtra : mma_extra(R == 8 ? 1 : 2)>,
+                            attention_join<T, E, R, f32 ? SimtShape<E>::kUnit : MmaShape<E>::kUnit,
+                                           f32 ? kSimtExtra : mma_extra(R == 8 ? 1 : 2)>,
                             dim3(adders + G * rows), dim3(kThreads), 0, s, a, rows, G, adders);
 }
 
@@ -876,6 +918,9 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
                                               max_pages, page_stride, head_stride, row_stride, dtype))
             return rc;
         if (B == 0) return NNOP_OK;
+        // the split's unit numbers times its CTAs stay within 64 bits
+        if ((double)B * (double)QH * (a.c.slots / 16 + 32) > 9e15)
+            return fail(NNOP_ERR_SHAPE, "paged_attention: too many slots in all");
         if (!q || !o || !lse || !workspace || (pages > 0 && (!k_cache || !v_cache)))
             return fail(NNOP_ERR_ARG, "paged_attention: NULL pointer");
         if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o))

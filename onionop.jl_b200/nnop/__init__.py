@@ -775,6 +775,8 @@ def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, si
     T = shape[2]
     QH, cb, qo = 0, 1, None
     if cos is not None:
+        if cos.dim() not in (2, 3):
+            raise NNopShapeError(-1, "cos/sin must have shape (B or 1, L, E)")
         cb, f32 = cos.shape[0], torch.float32
         if cos.shape == (cb, T, E) == sin.shape and cb in (1, B) and cos.dtype is f32 and sin.dtype is f32:
             cos, sin = cos.contiguous(), sin.contiguous()
