@@ -277,10 +277,15 @@ attention_simt(AttnArgs a) {
 // row (4 lanes read 64 bytes of each of 8 rows), and Q is laid out to match.  The
 // rows of Oᵀ may be any E order too: a lane loads 16 bytes of 4 V rows (8 lanes read
 // 128 bytes of a row) and pairs two keys' halves by byte permutes.  Sᵀ's
-// accumulators become Pᵀ's B fragments by movmatrix.  P goes in as the sum of two
-// 16-bit terms: rounded once to 16 bits it would cost as much accuracy as rounding
-// the result does.  f16: P is scaled by 2^14, which the running sum shares, so that
-// weights down to 2^-38 of the largest count.
+// accumulators become Pᵀ's B fragments by movmatrix.  P keeps fp32's bits: it goes in
+// as the sum of three bf16 terms (24 bits) or two f16 terms (22 bits, less than ex2's
+// own error away).  Rounded once to 16 bits it would cost as much accuracy as rounding
+// the result does.  Of 65536 bf16 results (16 sequences up to 8192) two terms (16 bits)
+// rounded 78 to another side than exact values do, three 47, products in fp32 34; the third
+// term takes 64 such sequences from 168 to 171 us (the launch alone), groups of 16 heads
+// from 111 to 119.
+// f16: P is scaled by 2^14, which the running sum shares, so that weights down to
+// 2^-38 of the largest count.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -314,6 +319,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
+// Two values rounded to T, and what the rounding left of them (rest_lo, rest_hi may be lo, hi).
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi, float& rest_lo, float& rest_hi) {
     if constexpr (std::is_same<T, __half>::value) {
         const __half2 h = __floats2half2_rn(lo, hi);
@@ -356,6 +362,7 @@ attention_mma(AttnArgs a) {
     constexpr int KW = E >= 32 ? 4 : 2, KC = E / (8 * KW);     // words per K load, loads per row
     constexpr int VW = E >= 64 ? 4 : E == 32 ? 2 : 1, VC = E / (16 * VW);
     constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
+    constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 3;
     __shared__ SplitShared sh;
     __shared__ float wm[4][8 * NT], wl[4][8 * NT];
     __shared__ __align__(16) float wacc[4][8 * NT][E];
@@ -556,7 +563,7 @@ attention_mma(AttnArgs a) {
                                 a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = d[n][t][i] * a.scale2;
                         }
             }
-            uint32_t b[NT][S::kTiles][2][2];      // Pᵀ: [16-bit term][key half]
+            uint32_t b[NT][S::kTiles][kTerms][2];      // Pᵀ: [16-bit term][key half]
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float mx[2] = {d[n][0][0], d[n][0][1]};
@@ -590,13 +597,12 @@ attention_mma(AttnArgs a) {
                 for (int t = 0; t < S::kTiles; ++t)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float p0 = fast_exp2(fmaf(d[n][t][i * 2], a.scale2, -base[n][0]));
-                        const float p1 = fast_exp2(fmaf(d[n][t][i * 2 + 1], a.scale2, -base[n][1]));
+                        float p0 = fast_exp2(fmaf(d[n][t][i * 2], a.scale2, -base[n][0]));
+                        float p1 = fast_exp2(fmaf(d[n][t][i * 2 + 1], a.scale2, -base[n][1]));
                         l[n][0] += p0;
                         l[n][1] += p1;
-                        float e0, e1, u0, u1;
-                        b[n][t][0][i] = transpose8x8(pack2<T>(p0, p1, e0, e1));
-                        b[n][t][1][i] = transpose8x8(pack2<T>(e0, e1, u0, u1));
+#pragma unroll
+                        for (int k = 0; k < kTerms; ++k) b[n][t][k][i] = transpose8x8(pack2<T>(p0, p1, p0, p1));
                     }
             }
 #pragma unroll
@@ -612,10 +618,10 @@ attention_mma(AttnArgs a) {
                         const uint32_t a2 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x5410);
                         const uint32_t a3 = __byte_perm(vr[t][2][c][j], vr[t][3][c][j], 0x7632);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][0][0], b[n][t][0][1]);
-                            mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][1][0], b[n][t][1][1]);
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int k = 0; k < kTerms; ++k)
+                                mma16816<T>(acc[n][c][j], a0, a1, a2, a3, b[n][t][k][0], b[n][t][k][1]);
                     }
                     if (!kWholeTiles && more) {
 #pragma unroll

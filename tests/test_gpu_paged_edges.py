@@ -1,0 +1,56 @@
+"""The paged key-value cache at its edges: precision that only a cancelling sum
+shows, values that are not finite, and shapes that take a kernel variant of their
+own.  Helpers and tolerances: test_gpu_paged.py (u = 2^-24, the half step of fp32)."""
+import math
+
+import numpy as np
+import pytest
+
+from _util import to_dev, to_np, torch_dtype
+from test_gpu_paged import U
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f32": U, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_probabilities_enter_the_sum_with_32_bits(dtype):
+    """Two keys whose values cancel to 2^-16 of themselves, so that o shows the bits of
+    the probabilities that the rounding of o hides elsewhere.
+
+    Scores are exact (one product of two 16-bit numbers; the scale is 1/4): 0 and -x, so
+    the weights are 1 and p = exp(-x).  p is off by ex2's 2^-22, by 2^-22 for what its
+    split into terms may drop, and by 4u·x for the rounding of its argument; v1 + p·v2 by
+    two half steps of its larger addend, twice (later terms are 2^-8 of it: 1/16 more);
+    the division and the rounding of o by their share of o, half a step of f16's smallest
+    (2^-25) where o is that small."""
+    import torch
+
+    import nnop
+    B, E = 256, 16
+    dt = torch_dtype(dtype)
+    rng = np.random.default_rng(50)
+    cast = lambda a: torch.from_numpy(np.asarray(a, np.float64)).to(dt).double().numpy()  # noqa: E731
+    xq, xk = cast(rng.uniform(0.3, 1.0, B)), cast(rng.uniform(0.3, 3.0, B))
+    if dtype == "f32":                       # a product that fits 24 bits there too
+        xq, xk = (np.round(a * 256) / 256 for a in (xq, xk))
+    x = xq * xk / 4
+    p = np.exp(-x)[:, None]
+    v1 = cast(rng.uniform(1, 2, (B, 512)))
+    v2 = cast(-v1 / p)
+    best = np.argsort(np.abs(v1 + p * v2), axis=1)[:, :E]
+    v1, v2 = np.take_along_axis(v1, best, 1), np.take_along_axis(v2, best, 1)
+    q, k, v = np.zeros((B, 1, 1, E)), np.zeros((B, 1, 16, E)), np.zeros((B, 1, 16, E))
+    q[:, 0, 0, 3], k[:, 0, 1, 3] = xq, -xk
+    v[:, 0, 0], v[:, 0, 1] = v1, v2
+    k[:, :, 2:] = v[:, :, 2:] = math.nan
+    table = torch.arange(B, device="cuda", dtype=torch.int32)[:, None]
+    o = nnop.paged_attention(to_dev(q, dtype), to_dev(k, dtype), to_dev(v, dtype), table,
+                             torch.full((B,), 2, device="cuda", dtype=torch.int32))
+    want = (v1 + p * v2) / (1 + p)
+    a2 = p * np.abs(v2)
+    tol = (a2 * (2.0 ** -21 + 4 * U * x[:, None]) + 4 * U * np.maximum(np.abs(v1), a2) * (1 + 2.0 ** -4)) / (1 + p)
+    tol += (HALF[dtype] + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "f16" else 0)
+    over = np.abs(to_np(o)[:, 0, 0] - want) / tol
+    assert over.max() <= 1, f"{over.max():.3g} times its tolerance"
