@@ -817,8 +817,13 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
                                 add[i] += fast_exp2(sc[j0 + i * kThreads] - lse2);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (j0 + i * kThreads < end) w[j0 + i * kThreads] = sum[i] + add[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = j0 + i * kThreads;
+                        if (j >= end) continue;
+                        // a row that is not finite gives its slots NaN, but none to those without a page
+                        if (add[i] != add[i] && a.c.offset(a.c.table + (int64_t)s.b * a.c.max_pages, j) < 0) add[i] = 0.f;
+                        if (add[i] != 0.f) w[j] = sum[i] + add[i];
+                    }
                 }
             }
         }

@@ -54,3 +54,27 @@ def test_probabilities_enter_the_sum_with_32_bits(dtype):
     tol += (HALF[dtype] + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "f16" else 0)
     over = np.abs(to_np(o)[:, 0, 0] - want) / tol
     assert over.max() <= 1, f"{over.max():.3g} times its tolerance"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("PS", [8, 16])
+@pytest.mark.parametrize("n", [45, 20000])
+def test_weights_of_a_row_that_is_not_finite(dtype, PS, n):
+    """One NaN score makes every attended slot's weight NaN; slots without a page are not
+    attended to and keep what they have, to the bit."""
+    import torch
+
+    import nnop
+    MP = -(-n // PS)
+    pages = np.arange(MP, dtype=np.int32)[None].copy()
+    pages[0, 1], pages[0, MP // 2], pages[0, -1] = -1, MP, 2 ** 31 - 1
+    kc, vc = (torch.randn(MP, 2, PS, 32, device="cuda").to(torch_dtype(dtype)) for _ in range(2))
+    kc[0, 1, 3, 5] = math.nan                       # slot 3 of the second head
+    q = torch.ones(1, 4, 1, 32, device="cuda", dtype=torch_dtype(dtype))
+    w = torch.full((1, 2, MP * PS), -0.0, device="cuda")
+    nnop.paged_attention(q, kc, vc, torch.from_numpy(pages).cuda(), torch.tensor([n], device="cuda", dtype=torch.int32),
+                         weights=w)
+    attended = np.isin(np.arange(MP * PS) // PS, [1, MP // 2, MP - 1], invert=True) & (np.arange(MP * PS) < n)
+    w = w.cpu().numpy()[0]
+    assert np.isnan(w[1, attended]).all() and (w[0, attended] > 0).all()
+    assert (w[:, ~attended].view(np.uint32) == 0x80000000).all()
