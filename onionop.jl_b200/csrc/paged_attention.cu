@@ -42,6 +42,8 @@ struct AttnArgs {
     float* scores;                 // [B][QH][slots], log2 domain (with weights)
 };
 
+// For what ends in 16 bits: exp2f without its results below 2^-126 (0 here), of weights
+// whose largest is 1.  fp32 and the weights' sums take exp2f, which has them.
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -195,7 +197,7 @@ attention_simt(AttnArgs a) {
                     mx = fmaxf(mx, m[r]);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    const float alpha = fast_exp2(m[r] - mx);
+                    const float alpha = exp2f(m[r] - mx);
                     m[r] = mx;
                     l[r] *= alpha;
 #pragma unroll
@@ -204,7 +206,7 @@ attention_simt(AttnArgs a) {
                 const float base = m[r] == -INFINITY ? 0.f : m[r];      // no score yet
 #pragma unroll
                 for (int g = 0; g < KG; ++g) {
-                    sc[g][r] = fast_exp2(sc[g][r] - base);
+                    sc[g][r] = exp2f(sc[g][r] - base);
                     l[r] += sc[g][r];
                 }
             }
@@ -244,7 +246,7 @@ attention_simt(AttnArgs a) {
             float sum = 0.f, ac = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = fast_exp2(wm[w][r] - base);
+                const float f = exp2f(wm[w][r] - base);
                 sum = fmaf(wl[w][r], f, sum);
                 ac = fmaf(wacc[w][r][e], f, ac);
             }
@@ -694,8 +696,8 @@ attention_mma(AttnArgs a) {
 // Joins two parts of a row: maximum (log2 domain), sum and what is weighed with them.
 __device__ __forceinline__ float2 join_two(float2 x, float2 y, float& fx, float& fy) {
     const float mx = fmaxf(x.x, y.x), base = mx == -INFINITY ? 0.f : mx;
-    fx = fast_exp2(x.x - base);
-    fy = fast_exp2(y.x - base);
+    fx = exp2f(x.x - base);
+    fy = exp2f(y.x - base);
     return make_float2(mx, x.y * fx + y.y * fy);
 }
 
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (j0 + i * kThreads < end && lse2 != -INFINITY)
-                                add[i] += fast_exp2(sc[j0 + i * kThreads] - lse2);
+                                add[i] += exp2f(sc[j0 + i * kThreads] - lse2);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {

@@ -78,3 +78,30 @@ def test_weights_of_a_row_that_is_not_finite(dtype, PS, n):
     w = w.cpu().numpy()[0]
     assert np.isnan(w[1, attended]).all() and (w[0, attended] > 0).all()
     assert (w[:, ~attended].view(np.uint32) == 0x80000000).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [2, 40000])
+def test_weights_below_the_smallest_normal_number(dtype, n):
+    """A key 95 below the others in score: its weight is exp(-95) / (n - 1), 5.5e-42 for two
+    keys.  fp32 holds it in steps of 2^-149, and so do o (fp32, where only that key has a
+    value) and the weights of every type.  Half a step each from exp, the division and
+    the sum over two heads: 4 steps; and the rounding of the score, 137·2u·ln 2 of it."""
+    import torch
+
+    import nnop
+    kc, vc = (torch.zeros(1, 1, n, 16, device="cuda", dtype=torch_dtype(dtype)) for _ in range(2))
+    kc[0, 0, 1, 2] = -95.0
+    big = {"f32": 2.0 ** 126, "bf16": 2.0 ** 126, "f16": 0.0}[dtype]
+    vc[0, 0, 1] = big
+    q = torch.zeros(1, 2, 1, 16, device="cuda", dtype=torch_dtype(dtype))
+    q[..., 2] = 4.0                                 # the scale is 1/4
+    w = torch.zeros(1, 1, n, device="cuda")
+    o = nnop.paged_attention(q, kc, vc, torch.zeros(1, 1, device="cuda", dtype=torch.int32),
+                             torch.tensor([n], device="cuda", dtype=torch.int32), weights=w)
+    p = math.exp(-95) / (n - 1)
+    assert abs(float(w[0, 0, 1]) - 2 * p) <= 4 * 2.0 ** -149 + 2 * p * 200 * U
+    assert torch.allclose(w[0, 0, 2:], torch.tensor(2 / (n - 1), device="cuda"), rtol=1e-5)
+    if dtype == "f32":
+        # the numerator's exp(-95) alone is in steps of 2^-149
+        assert np.abs(to_np(o) - p * big).max() <= 2 * 2.0 ** -149 * big / (n - 1) + p * big * 200 * U
