@@ -37,9 +37,10 @@ struct AttnArgs {
     int QH, KH, group, tiles;      // tiles: head tiles of R rows per KV head
     float scale2;                  // scale · log2(e)
     int4* join;                    // [kMaxCtas] (b, head tile, CTAs, -) of a split that starts in CTA c; CTAs = 0: none
-    float2* part_ml;               // [2·kMaxCtas][R] maximum (log2 domain), sum
+    float2* part_ml;               // [2·kMaxCtas][R] maximum (scaled, log2 domain), sum of exp2(s·scale2 − maximum)
     float* part_acc;               // [2·kMaxCtas][R][E]
-    float* scores;                 // [B][QH][slots], log2 domain (with weights)
+    float* scores;                 // [B][QH][slots] q·k, unscaled (with weights)
+    float2* row_ml;                // [B][QH] as part_ml, of a row that lies in one CTA (with weights)
 };
 
 // For what ends in 16 bits: exp2f without its results below 2^-126 (0 here), of weights
@@ -55,7 +56,10 @@ template <typename T, int E>
 __device__ __forceinline__ void write_row(const AttnArgs& a, int64_t b, int qh, int e, float acc, float m, float l) {
     const int64_t row = b * a.QH + qh;
     static_cast<T*>(a.o)[row * E + e] = from_f<T>(l > 0.f || l != l ? acc / l : 0.f);
-    if (e == 0) a.lse[row] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (e == 0) {
+        a.lse[row] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (a.row_ml != nullptr) a.row_ml[row] = make_float2(m, l);
+    }
 }
 
 // Sequences of length 0 have no unit: their rows are written here.
@@ -108,7 +112,7 @@ attention_simt(AttnArgs a) {
         for (int i = threadIdx.x; i < R * E; i += kThreads)
             qs[i / E][i % E] = i / E < rows ? static_cast<const float*>(a.q)[((int64_t)s.b * a.QH + qh0) * E + i] : 0.f;
         __syncthreads();
-        float m[R], l[R], acc[R][COLS];
+        float m[R], l[R], acc[R][COLS];      // m: maximum of the unscaled scores
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             m[r] = -INFINITY;
@@ -175,7 +179,7 @@ attention_simt(AttnArgs a) {
                     float x = sc[g][r];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    sc[g][r] = here[g] >= 0 ? x * a.scale2 : -INFINITY;
+                    sc[g][r] = here[g] >= 0 ? x : -INFINITY;
                 }
             if (a.scores != nullptr && sub == 0) {
 #pragma unroll
@@ -197,16 +201,16 @@ attention_simt(AttnArgs a) {
                     mx = fmaxf(mx, m[r]);
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    const float alpha = exp2f(m[r] - mx);
+                    const float alpha = exp2f(__fmul_rn(m[r], a.scale2) - __fmul_rn(mx, a.scale2));
                     m[r] = mx;
                     l[r] *= alpha;
 #pragma unroll
                     for (int i = 0; i < COLS; ++i) acc[r][i] *= alpha;
                 }
-                const float base = m[r] == -INFINITY ? 0.f : m[r];      // no score yet
+                const float base = m[r] == -INFINITY ? 0.f : __fmul_rn(m[r], a.scale2);      // -Inf: no score yet
 #pragma unroll
                 for (int g = 0; g < KG; ++g) {
-                    sc[g][r] = exp2f(sc[g][r] - base);
+                    sc[g][r] = exp2f(fmaf(sc[g][r], a.scale2, -base));
                     l[r] += sc[g][r];
                 }
             }
@@ -228,7 +232,7 @@ attention_simt(AttnArgs a) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
             if (lane == 0) {
-                wm[warp][r] = m[r];
+                wm[warp][r] = __fmul_rn(m[r], a.scale2);
                 wl[warp][r] = l[r];
             }
             if (lane * COLS < E) {
@@ -562,7 +566,7 @@ attention_mma(AttnArgs a) {
                         for (int i = 0; i < 4; ++i) {
                             const int key = key0 + t * 16 + i / 2 * 8 + gid, r = (tile0 + n) * 8 + 2 * sub + i % 2;
                             if (key < end && r < rows)
-                                a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = d[n][t][i] * a.scale2;
+                                a.scores[((int64_t)s.b * a.QH + qh0 + r) * a.c.slots + key] = d[n][t][i];
                         }
             }
             uint32_t b[NT][S::kTiles][kTerms][2];      // Pᵀ: [16-bit term][key half]
@@ -704,8 +708,8 @@ __device__ __forceinline__ float2 join_two(float2 x, float2 y, float& fx, float&
 // Part i of a split that CTA c has the first part of lies in slot 2(c + i), the first in 2c + 1.
 __device__ __forceinline__ int part_slot(int c, int i) { return 2 * (c + i) + (i == 0 ? 1 : 0); }
 
-// log2 of the sum of a row's parts, by a warp.
-__device__ __forceinline__ float join_lse2(const float2* part_ml, int R, int c, int parts, int r) {
+// Maximum and sum of a row from its parts, by a warp.
+__device__ __forceinline__ float2 join_ml(const float2* part_ml, int R, int c, int parts, int r) {
     const int lane = threadIdx.x & 31;
     float2 x = make_float2(-INFINITY, 0.f);
     float f0, f1;
@@ -713,14 +717,14 @@ __device__ __forceinline__ float join_lse2(const float2* part_ml, int R, int c, 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         x = join_two(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)), f0, f1);
-    return x.y > 0.f || x.y != x.y ? x.x + log2f(x.y) : -INFINITY;
+    return x;
 }
 
 // Second launch.  The last rows·ctas blocks: row j mod rows of the (sequence, head tile)
 // whose first part CTA j / rows wrote, each group of E/4 threads taking some of the
 // parts.  The `adders` blocks in front (with weights): weights[b][kv head][j] += Σ over the
-// group of exp(s_j − lse) for a share of the slots; a split row's lse comes from its
-// parts again, so that both run at once.
+// group of exp(s_j − maximum) / sum for a share of the slots; a split row's maximum and sum
+// come from its parts again, so that both run at once.
 template <typename T, int E, int R, int kUnit, int kExtra>
 __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int rows, int ctas, int adders) {
     constexpr int LE = E / 4;                             // lanes per row of 16-byte vectors
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
         struct {
             SplitShared split;
             int first[32], last[32];      // CTAs with the parts of a query head
-            float lse2[32];
+            float2 row[32];               // its maximum, and 1 / its sum (0: no score)
         } w;
     } sh;
     const int t = threadIdx.x;
@@ -803,20 +807,21 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
                         __syncthreads();
                         for (int g = t / 32; g < n; g += kThreads / 32) {
                             const int first = sh.w.first[g], parts = sh.w.last[g] - first + 1;
-                            const float lse2 = parts == 1 ? a.lse[row0 + g0 + g] * kLog2e
-                                                          : join_lse2(a.part_ml, R, first, parts, (g0 + g) % R);
-                            if (t % 32 == 0) sh.w.lse2[g] = lse2;
+                            const float2 x = parts == 1 ? a.row_ml[row0 + g0 + g]
+                                                        : join_ml(a.part_ml, R, first, parts, (g0 + g) % R);
+                            if (t % 32 == 0)
+                                sh.w.row[g] = x.y == 0.f ? make_float2(0.f, 0.f) : make_float2(x.x, 1.f / x.y);
                         }
                         __syncthreads();
                     }
                     float add[4] = {0.f, 0.f, 0.f, 0.f};
                     for (int g = 0; g < n; ++g) {
-                        const float lse2 = sh.w.lse2[g];
+                        const float2 x = sh.w.row[g];
                         const float* sc = a.scores + (row0 + g0 + g) * a.c.slots;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (j0 + i * kThreads < end && lse2 != -INFINITY)
-                                add[i] += exp2f(sc[j0 + i * kThreads] - lse2);
+                            if (j0 + i * kThreads < end) 
+                                add[i] = fmaf(exp2f(fmaf(sc[j0 + i * kThreads], a.scale2, -x.x)), x.y, add[i]);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -842,7 +847,7 @@ int rows_per_tile(int64_t group, int dtype) {
 }
 
 struct Layout {
-    size_t join, ml, acc, scores, bytes;
+    size_t join, ml, acc, scores, rows, bytes;
 };
 Layout layout(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t slots, bool weights, int dtype) {
     const size_t R = rows_per_tile(QH / KH, dtype);
@@ -851,7 +856,8 @@ Layout layout(int64_t E, int64_t QH, int64_t KH, int64_t B, int64_t slots, bool 
     w.ml = align256(sizeof(int4) * kMaxCtas);
     w.acc = w.ml + align256(sizeof(float2) * 2 * kMaxCtas * R);
     w.scores = w.acc + align256(sizeof(float) * 2 * kMaxCtas * R * E);
-    w.bytes = w.scores + (weights ? align256(sizeof(float) * (size_t)B * QH * slots) : 0);
+    w.rows = w.scores + (weights ? align256(sizeof(float) * (size_t)B * QH * slots) : 0);
+    w.bytes = w.rows + (weights ? align256(sizeof(float2) * (size_t)B * QH) : 0);
     return w;
 }
 
@@ -961,6 +967,7 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
         a.part_ml = reinterpret_cast<float2*>(base + w.ml);
         a.part_acc = reinterpret_cast<float*>(base + w.acc);
         a.scores = weights ? reinterpret_cast<float*>(base + w.scores) : nullptr;
+        a.row_ml = weights ? reinterpret_cast<float2*>(base + w.rows) : nullptr;
         const cudaStream_t s = (cudaStream_t)stream;
         const float sc = (float)(1.0 / std::sqrt((double)E));
         // scale rounded to the dtype, as flash_attention has it

@@ -105,3 +105,24 @@ def test_weights_below_the_smallest_normal_number(dtype, n):
     if dtype == "f32":
         # the numerator's exp(-95) alone is in steps of 2^-149
         assert np.abs(to_np(o) - p * big).max() <= 2 * 2.0 ** -149 * big / (n - 1) + p * big * 200 * U
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [48, 5000])
+def test_weights_of_far_scores(dtype, n):
+    """Equal scores s of about 2000 (exact: the scale is 1/4): every weight is 1/n, whatever
+    the rounding of s·log2(e) (1.7e-4 in a weight) that weight and sum share.  Off by ex2's
+    2^-22 in both, the division's and the sum's (80 + n/16)·u."""
+    import torch
+
+    import nnop
+    B = 16
+    k = np.zeros((B, 1, n, 16))
+    k[:, 0, :, 0] = 125.0 + np.arange(B)[:, None] / 16 * 3
+    q = np.zeros((B, 1, 1, 16))
+    q[..., 0] = 64.0
+    w = torch.zeros(B, 1, n, device="cuda")
+    nnop.paged_attention(to_dev(q, dtype), to_dev(k, dtype), to_dev(np.zeros_like(k), dtype),
+                         torch.arange(B, device="cuda", dtype=torch.int32)[:, None],
+                         torch.full((B,), n, device="cuda", dtype=torch.int32), weights=w)
+    assert np.abs(to_np(w) * n - 1).max() <= 2 * 2.0 ** -22 + 4 * U + (80 + n / 16) * U
