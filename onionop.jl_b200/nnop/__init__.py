@@ -697,7 +697,7 @@ def llama_rope(q, k, *, cos, sin):
 # call's: plain checks in the order of a valid call, the device as its index (-1 on the
 # CPU), messages made only when they are needed.
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # a torch without CUDA has none; no call gets that far there
 _workspace_bytes = functools.lru_cache(maxsize=1024)(lib.nnop_paged_attention_fwd_workspace_size)
 
 
