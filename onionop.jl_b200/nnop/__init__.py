@@ -752,8 +752,10 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _on(dev, fn, *args):
-    """Calls the library on device ``dev`` with its current stream last."""
+def _on(dev, written, fn, *args):
+    """Calls the library on device ``dev`` with its current stream last.  ``written``: the
+    caller's tensors it changes in place, whose version torch is told to count up, so that
+    a backward pass that saved one of them refuses to go on."""
     if dev == torch.cuda.current_device():
         status = fn(*args, _raw_stream(dev))
     else:
@@ -761,6 +763,8 @@ def _on(dev, fn, *args):
             status = fn(*args, _raw_stream(dev))
     if status:
         check(status)
+    if written:
+        torch.autograd.graph.increment_version(written)
 
 
 def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, sin, n_new):
@@ -798,7 +802,7 @@ def _paged_append(name, q, k, v, k_cache, v_cache, block_table, lengths, cos, si
         n_new = n_new.contiguous()
     k, v, lengths, block_table = _aligned(k), _aligned(v), lengths.contiguous(), block_table.contiguous()
     new_lengths = torch.empty_like(lengths)
-    _on(dev, lib.nnop_paged_append, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos), _ptr(sin), _ptr(n_new), _ptr(qo),
+    _on(dev, (k_cache, v_cache), lib.nnop_paged_append, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(cos), _ptr(sin), _ptr(n_new), _ptr(qo),
         k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), new_lengths.data_ptr(), E, T,
         QH, KH, B, cb, *cache, _dtype_id(k_cache))
     return qo, new_lengths
@@ -850,7 +854,7 @@ def _paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None)
     ws_bytes = _workspace_bytes(E, QH, KH, B, cache[1], cache[2], weigh, dt)
     o, lse = torch.empty_like(q), q.new_empty((B, QH, 1), dtype=torch.float32)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
-    _on(dev, lib.nnop_paged_attention_fwd, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+    _on(dev, (weights,) if weigh else (), lib.nnop_paged_attention_fwd, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
         lengths.data_ptr(), weights.data_ptr() if weigh else None, o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws_bytes,
         E, QH, KH, B, *cache, dt)
     return o, lse
@@ -900,7 +904,7 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
     block_table, new_table = block_table.contiguous(), new_table.contiguous()
     new_lengths = torch.empty_like(lengths)
     new_weights, kept = weights.new_empty((B, KH, slots)), lengths.new_empty((B, KH, budget))
-    _on(dev, lib.nnop_paged_evict, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), new_table.data_ptr(),
+    _on(dev, (k_cache, v_cache), lib.nnop_paged_evict, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), new_table.data_ptr(),
         lengths.data_ptr(), weights.data_ptr(), new_lengths.data_ptr(), new_weights.data_ptr(), kept.data_ptr(), E, KH, B,
         *cache[:3], new_table.shape[1], *cache[3:], budget, recent, _dtype_id(k_cache))
     return new_lengths, new_weights, kept

@@ -126,3 +126,44 @@ def test_weights_of_far_scores(dtype, n):
                          torch.arange(B, device="cuda", dtype=torch.int32)[:, None],
                          torch.full((B,), n, device="cuda", dtype=torch.int32), weights=w)
     assert np.abs(to_np(w) * n - 1).max() <= 2 * 2.0 ** -22 + 4 * U + (80 + n / 16) * U
+
+
+def _state(MP=3, n=(20, 5)):
+    """q, the new rows k and v, pools, a table, lengths and weights of two sequences."""
+    import torch
+    B, QH, KH, E, PS = 2, 4, 2, 64, 16
+    r = lambda *s: torch.randn(*s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    kc, vc = r(2 * B * MP, KH, PS, E), r(2 * B * MP, KH, PS, E)
+    t = torch.arange(2 * B * MP, device="cuda", dtype=torch.int32).view(2, B, MP)
+    return (r(B, QH, 1, E), r(B, KH, 1, E), r(B, KH, 1, E), kc, vc, t,
+            torch.tensor(n, device="cuda", dtype=torch.int32), torch.rand(B, KH, MP * PS, device="cuda"))
+
+
+def test_writes_count_as_changes_in_place():
+    """A backward pass that saved a pool or the weights does not go on with what a call
+    has written there since; tensors of inference mode, which have no version, work."""
+    import torch
+
+    import nnop
+    q, k, v, kc, vc, t, n, w = _state()
+    cos, sin = nnop.LlamaRotaryEmbedding(64)(n[:, None].float())
+    calls = [(lambda: nnop.paged_append(k, v, kc, vc, t[0], n), (kc, vc)),
+             (lambda: nnop.paged_append_rope(q, k, v, kc, vc, t[0], n, cos=cos, sin=sin), (kc, vc)),
+             (lambda: nnop.paged_attention(q, kc, vc, t[0], n, weights=w), (w,)),
+             (lambda: nnop.paged_evict(kc, vc, t[0], t[1], n, w, budget=4), (kc, vc))]
+    for call, written in calls:
+        for x in written:
+            y = torch.ones_like(x, requires_grad=True)
+            z = (x[:1] * y[:1]).sum()                # saves a view of x
+            call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                z.backward()
+    y = torch.ones_like(kc, requires_grad=True)
+    z = (kc * y).sum()
+    nnop.paged_attention(q, kc, vc, t[0], n, weights=w)      # only reads the pools
+    z.backward()
+    with torch.inference_mode():
+        q, k, v, kc, vc, t, n, w = _state()
+        nnop.paged_append(k, v, kc, vc, t[0], n)
+        nnop.paged_attention(q, kc, vc, t[0], n, weights=w)
+        nnop.paged_evict(kc, vc, t[0], t[1], n, w, budget=4)
