@@ -29,6 +29,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import (BF16, F16, F32, NNopError, NNopShapeError, check, lib)
 
@@ -744,6 +745,10 @@ def _no_grad(name, *ts):
         for t in ts:
             if t is not None and t.requires_grad:
                 raise NNopError(-3, f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:           # inside forward_ad.dual_level()
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NNopError(-3, f"{name} has no forward-mode derivative: call it on tensors without a tangent")
 
 
 def _aligned(t):

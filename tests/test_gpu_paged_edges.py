@@ -167,3 +167,23 @@ def test_writes_count_as_changes_in_place():
         nnop.paged_append(k, v, kc, vc, t[0], n)
         nnop.paged_attention(q, kc, vc, t[0], n, weights=w)
         nnop.paged_evict(kc, vc, t[0], t[1], n, w, budget=4)
+
+
+def test_tangents_are_refused():
+    """A forward-mode tangent would be dropped without a word."""
+    import torch
+    from torch.autograd import forward_ad
+
+    import nnop
+    q, k, v, kc, vc, t, n, w = _state()
+    cos, sin = nnop.LlamaRotaryEmbedding(64)(n[:, None].float())
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for call in (lambda: nnop.paged_append(dual(k), v, kc, vc, t[0], n),
+                     lambda: nnop.paged_append_rope(dual(q), k, v, kc, vc, t[0], n, cos=cos, sin=sin),
+                     lambda: nnop.paged_attention(q, kc, dual(vc), t[0], n),
+                     lambda: nnop.paged_attention(q, kc, vc, t[0], n, weights=dual(w)),
+                     lambda: nnop.paged_evict(dual(kc), vc, t[0], t[1], n, w, budget=4)):
+            with pytest.raises(nnop.NNopError, match="no forward-mode derivative"):
+                call()
+        nnop.paged_attention(q, kc, vc, t[0], n, weights=w)
