@@ -508,7 +508,7 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
  * of block_table are only read (another sequence may share them) and are the
  * caller's to release.
  *   new_table [B][new_max_pages] int32, budget <= new_max_pages*page_size;
- *   its pages are distinct and none is a page that block_table names (else the
+ *   both tables have at most 2^31 - 8192 slots per sequence here; its pages are distinct and none is a page that block_table names (else the
  *   rows copied are left open).
  *   weights [B][KH][max_pages*page_size] f32;
  *   new_weights [B][KH][new_max_pages*page_size] f32: the kept slots' weights,

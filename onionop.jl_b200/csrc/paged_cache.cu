@@ -185,6 +185,10 @@ constexpr size_t kHistBytes = sizeof(int) * kDigits * kBins;
 constexpr int kMostKeys = 48 * 1024;                         // of a CTA's share in shared memory
 
 constexpr int kMostCtas = 8;                                 // of a cluster
+// The kernel counts slots with 32-bit numbers in steps of up to its whole cluster, and the
+// last step goes past the end.
+constexpr int64_t kMostEvictSlots = ((int64_t)1 << 31) - kMostCtas * kSelectThreads;
+static_assert(kMostCtas * kSelectThreads >= 4 * kSelectThreads, "a thread takes four keys of its CTA's share a step");
 
 // Sum over the lanes in front.
 __device__ __forceinline__ int warp_sum_before(int n) {
@@ -542,9 +546,9 @@ int nnop_paged_evict(void* k_cache, void* v_cache, const int32_t* block_table, c
         if (const int rc = paged::check_cache("paged_evict", a.c, block_table, lengths, E, KH, B, pages, page_size,
                                               max_pages, page_stride, head_stride, row_stride, dtype))
             return rc;
-        const int64_t most = ((int64_t)1 << 31) - 1024;
-        if (new_max_pages < 0 || new_max_pages > most || new_max_pages * page_size > most)
-            return fail(NNOP_ERR_SHAPE, "paged_evict: more than 2^31 - 1024 slots per sequence");
+        const int64_t most = paged::kMostEvictSlots;
+        if (new_max_pages < 0 || new_max_pages > most || new_max_pages * page_size > most || a.c.slots > most)
+            return fail(NNOP_ERR_SHAPE, "paged_evict: more than 2^31 - 8192 slots per sequence");
         if (budget < 0 || recent < 0 || recent > budget || budget > new_max_pages * page_size)
             return fail(NNOP_ERR_SHAPE, "paged_evict: 0 <= recent <= budget <= slots of the new table");
         if (B == 0) return NNOP_OK;

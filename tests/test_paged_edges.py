@@ -5,6 +5,8 @@ import pathlib
 import subprocess
 import sys
 
+from test_paged import _append, _attend, _evict
+
 ROOT = pathlib.Path(__file__).resolve().parent.parent
 
 
@@ -26,3 +28,19 @@ else:
     env = dict(os.environ, PYTHONPATH=str(ROOT / "onionop.jl_b200"), CUDA_VISIBLE_DEVICES="")
     r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-1000:]
+
+
+def test_evict_refuses_what_its_counters_do_not_hold():
+    """The choice of slots goes through a row in steps of up to 8192 slots (a cluster of 8
+    CTAs of 1024 threads) with 32-bit counters: the last step ends past the last slot, so
+    8192 slots fewer than 2^31 are the most.  The calls at the limit are refused for a
+    missing array, none is launched."""
+    from nnop._lib import lib
+    assert 2 ** 31 - 8192 - 1 + 8192 <= 2 ** 31 - 1
+    for pages in ({"MP": 2 ** 21 - 1}, {"NP": 2 ** 21 - 1}, {"NP": 2 ** 21 - 7}, {"MP": 2 ** 21 - 7}):
+        assert _evict(lib, PS=1024, kept=None, **pages) == -1, pages
+        assert b"2^31 - 8192 slots" in lib.nnop_last_error()
+    for pages in ({"MP": 2 ** 21 - 8}, {"NP": 2 ** 21 - 8}):
+        assert _evict(lib, PS=1024, kept=None, **pages) == -3
+    # the other calls' counters step by at most 1024
+    assert _append(lib, PS=1024, MP=2 ** 21 - 1, new=None) == -3 and _attend(lib, PS=1024, MP=2 ** 21 - 1, lse=None) == -3
