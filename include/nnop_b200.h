@@ -450,7 +450,7 @@ int nnop_llama_rope_cos_sin(const float* position_ids, float* cos_t, float* sin_
  * [0, T]) of k and v goes to slot lengths[b] + t of sequence b.  Rows past the
  * table's last slot are dropped.  Nothing else of the pools is written.
  *   k, v [B][KH][T][E]; new_lengths [B] = min(lengths + n_new, slots), not
- *   the array `lengths` itself.
+ *   the array `lengths` or `n_new` itself.
  *   cos_t, sin_t [cos_batch][T][E] f32 (cos_batch = 1 or B) or both NULL: k is
  *   rotated on its way as nnop_llama_rope rotates it, bit for bit, and with
  *   QH > 0 so are the queries q [B][QH][T][E] into q_out (all T of them).

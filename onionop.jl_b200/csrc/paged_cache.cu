@@ -510,8 +510,9 @@ int nnop_paged_append(const void* q, const void* k, const void* v, const float* 
         if (cos_t && cos_batch != B && cos_batch != 1)
             return fail(NNOP_ERR_SHAPE, "paged_append: cos/sin batch must equal the batch or be 1");
         if (B == 0) return NNOP_OK;
-        if (!new_lengths || new_lengths == lengths || (T > 0 && (!k || !v)) || (pages > 0 && (!k_cache || !v_cache)))
-            return fail(NNOP_ERR_ARG, "paged_append: NULL pointer, or new_lengths is lengths");
+        if (!new_lengths || new_lengths == lengths || new_lengths == n_new || (T > 0 && (!k || !v)) ||
+            (pages > 0 && (!k_cache || !v_cache)))
+            return fail(NNOP_ERR_ARG, "paged_append: NULL pointer, or new_lengths is lengths or n_new");
         if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
             return fail(NNOP_ERR_ALIGN, "paged_append: tensors must be 16-byte aligned");
         a.q = q;

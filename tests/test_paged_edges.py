@@ -44,3 +44,14 @@ def test_evict_refuses_what_its_counters_do_not_hold():
         assert _evict(lib, PS=1024, kept=None, **pages) == -3
     # the other calls' counters step by at most 1024
     assert _append(lib, PS=1024, MP=2 ** 21 - 1, new=None) == -3 and _attend(lib, PS=1024, MP=2 ** 21 - 1, lse=None) == -3
+
+
+def test_append_refuses_to_write_the_lengths_over_the_counts():
+    """Other blocks still read n_new while new_lengths is written."""
+    import ctypes as C
+
+    from nnop._lib import lib
+    a, b = C.c_void_p(4096), C.c_void_p(8192)
+    call = lambda n_new, new: lib.nnop_paged_append(None, a, a, None, None, n_new, None, a, a, a, a, new,  # noqa: E731
+                                                    64, 1, 0, 2, 1, 1, 4, 16, 2, 2048, 1024, 64, 2, None)
+    assert call(b, b) == -3 and b"lengths or n_new" in lib.nnop_last_error()
