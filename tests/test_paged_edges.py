@@ -2,6 +2,7 @@
 what the C ABI refuses at its limits, and the documented bindings."""
 import os
 import pathlib
+import re
 import subprocess
 import sys
 
@@ -55,3 +56,46 @@ def test_append_refuses_to_write_the_lengths_over_the_counts():
     call = lambda n_new, new: lib.nnop_paged_append(None, a, a, None, None, n_new, None, a, a, a, a, new,  # noqa: E731
                                                     64, 1, 0, 2, 1, 1, 4, 16, 2, 2048, 1024, 64, 2, None)
     assert call(b, b) == -3 and b"lengths or n_new" in lib.nnop_last_error()
+
+
+def _split(text):
+    """The arguments of a Julia call: what lies between commas outside all brackets."""
+    parts, depth, last = [], 0, 0
+    for i, c in enumerate(text):
+        depth += (c in "([{") - (c in ")]}")
+        if c == "," and depth == 0:
+            parts.append(text[last:i])
+            last = i + 1
+    return [p.strip() for p in [*parts, text[last:]] if p.strip()]
+
+
+def _ccalls():
+    """(name, return type, argument types, arguments) of each ccall in the documented binding."""
+    text = (ROOT / "INTEGRATION.md").read_text()
+    for block in re.findall(r"```julia\n(.*?)```", text, re.S):
+        block = re.sub(r"#.*", "", block)
+        for m in re.finditer(r"ccall\(", block):
+            depth, i = 1, m.end()
+            while depth:
+                depth += (block[i] == "(") - (block[i] == ")")
+                i += 1
+            target, result, types, *args = _split(block[m.end():i - 1])
+            yield re.match(r"\(:(\w+), libnnop\)", target)[1], result, _split(types[1:-1]), args
+
+
+def test_documented_bindings_have_the_signatures_of_the_library():
+    """Julia's ccall pairs types and arguments as they are written: one argument for each
+    type, no splat.  The paged calls are all bound."""
+    import ctypes as C
+
+    from nnop._lib import SIGNATURES
+    kinds = {"Int64": C.c_int64, "Cint": C.c_int, "Csize_t": C.c_size_t, "Float32": C.c_float, "Cstring": C.c_char_p}
+    of = lambda t: C.c_void_p if re.fullmatch(r"(Cu)?Ptr\{\w+\}", t) else kinds[t]  # noqa: E731
+    seen = set()
+    for name, result, types, args in _ccalls():
+        res, argtypes = SIGNATURES[name]
+        assert not any(a.endswith("...") for a in args), name
+        assert len(types) == len(args) == len(argtypes), name
+        assert [of(t) for t in types] == list(argtypes) and of(result) == res, name
+        seen.add(name)
+    assert {n for n in SIGNATURES if n.startswith("nnop_paged")} <= seen
