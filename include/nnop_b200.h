@@ -448,7 +448,8 @@ int nnop_llama_rope_cos_sin(const float* position_ids, float* cos_t, float* sin_
 /*
  * Appends new rows: row t < n_new[b] (n_new NULL: all T; taken as within
  * [0, T]) of k and v goes to slot lengths[b] + t of sequence b.  Rows past the
- * table's last slot are dropped.  Nothing else of the pools is written.
+ * table's last slot are dropped: new_lengths then falls short of lengths +
+ * n_new.  Nothing else of the pools is written.
  *   k, v [B][KH][T][E]; new_lengths [B] = min(lengths + n_new, slots), not
  *   the array `lengths` or `n_new` itself.
  *   cos_t, sin_t [cos_batch][T][E] f32 (cos_batch = 1 or B) or both NULL: k is
@@ -507,9 +508,13 @@ int nnop_paged_attention_fwd(const void* q, const void* k_cache, const void* v_c
  * order, to slots 0, 1, ... of new_table's pages in the same pools; the pages
  * of block_table are only read (another sequence may share them) and are the
  * caller's to release.
- *   new_table [B][new_max_pages] int32, budget <= new_max_pages*page_size;
- *   both tables have at most 2^31 - 8192 slots per sequence here; its pages are distinct and none is a page that block_table names (else the
- *   rows copied are left open).
+ *   new_table [B][new_max_pages] int32, budget <= new_max_pages*page_size; its
+ *   pages are distinct and none is a page that block_table names (else the
+ *   rows copied are left open).  Both tables have at most 2^31 - 8192 slots per
+ *   sequence here.  A sequence over its budget has `budget` slots in use
+ *   afterwards: a table that is appended to needs room for more, up to the next
+ *   eviction.  A kept slot that block_table has no page for leaves its new
+ *   slot's row as it was: every slot in use should have a page.
  *   weights [B][KH][max_pages*page_size] f32;
  *   new_weights [B][KH][new_max_pages*page_size] f32: the kept slots' weights,
  *   0 behind them; new_lengths [B] = min(lengths, budget);

@@ -821,7 +821,9 @@ def paged_append(k, v, k_cache, v_cache, block_table, lengths, *, n_new=None):
     ``k_cache``, ``v_cache`` (P, KH, PS, E): the pools, written in place; any
     strides with E contiguous, the same for both.  ``block_table`` (B, MP) int32:
     the page of each run of PS slots; an entry outside [0, P) is no page and rows
-    meant for it are dropped, as are rows past the table's MP·PS slots.
+    meant for it are dropped (their slots count as used, and are not attended to),
+    as are rows past the table's MP·PS slots: the new lengths then fall short of
+    ``lengths + n_new``.
     ``n_new`` (B,) int32: how many of the T rows are tokens, for a padded batch
     (default all).  A page that is written belongs to one sequence."""
     return _paged_append("paged_append", None, k, v, k_cache, v_cache, block_table, lengths, None, None, n_new)[1]
@@ -886,7 +888,11 @@ def paged_evict(k_cache, v_cache, block_table, new_table, lengths, weights, *, b
 
     The kept rows are copied in order to the pages of ``new_table`` (B, MP')
     int32 in the same pools; those pages are distinct and none of them is read
-    by this call.  The old pages are only read.  Returns ``(new_lengths (B,),
+    by this call.  The old pages are only read.  ``new_table`` has room for
+    ``budget`` slots and, where it becomes the sequence's table, for what is
+    appended before the next eviction: rows past its last slot are dropped.  A
+    kept slot that ``block_table`` has no page for leaves its new slot's row as
+    it was, so every slot in use has a page.  Returns ``(new_lengths (B,),
     new_weights (B, KH, MP'·PS), kept (B, KH, budget))``: the kept slots' weights
     (0 behind them) and their old slots, ascending (-1 behind them)."""
     name = "paged_evict"

@@ -187,3 +187,41 @@ def test_tangents_are_refused():
             with pytest.raises(nnop.NNopError, match="no forward-mode derivative"):
                 call()
         nnop.paged_attention(q, kc, vc, t[0], n, weights=w)
+
+
+@pytest.mark.parametrize("budget", [32, 40])
+def test_documented_decode_loop_keeps_its_tokens(budget):
+    """The decode step of INTEGRATION.md as it stands there, over several evictions: every
+    token lands behind the ones before it and is attended to, none is dropped."""
+    import pathlib
+    import re
+
+    import torch
+
+    import nnop
+    text = (pathlib.Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    setup, step = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "held" in b]
+    B, QH, KH, E, page_size, recent = 2, 4, 2, 64, 16, 8
+    r = lambda h: torch.randn(B, h, 1, E, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    ns = dict(torch=torch, nnop=nnop, B=B, KH=KH, page_size=page_size, budget=budget, recent=recent,
+              free=torch.randperm(64, device="cuda").int(), emb=nnop.LlamaRotaryEmbedding(E))
+    ns["k_cache"], ns["v_cache"] = (torch.full((64, KH, page_size, E), math.nan, device="cuda", dtype=torch.bfloat16)
+                                    for _ in range(2))
+    exec(setup, ns)
+    evictions, held = 0, 0
+    for pos in range(150):
+        q, k, v = r(QH), r(KH), r(KH)
+        ns.update(q=q, k=k, v=v, positions=torch.full((B,), pos, device="cuda", dtype=torch.int32))
+        exec(step, ns)
+        held += 1
+        assert not ns["o"].isnan().any()
+        evicted = ns["lengths"].tolist() != [held] * B
+        if evicted:
+            assert ns["lengths"].tolist() == [budget] * B
+            evictions, held = evictions + 1, budget
+        # the newest token, among the last `recent` even after an eviction
+        table, at = ns["table"], held - 1
+        for b in range(B):
+            assert torch.equal(ns["v_cache"][table[b, at // page_size], :, at % page_size], v[b, :, 0])
+        assert (ns["weights"][:, :, at] > 0).all()
+    assert evictions >= 3
