@@ -787,21 +787,23 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
         if (s.h % a.tiles == 0) {
             const int64_t row0 = (int64_t)s.b * a.QH + kvh * a.group;
             float* w = a.weights + ((int64_t)s.b * a.KH + kvh) * a.c.slots;
-            for (int g0 = 0; g0 < a.group; g0 += 32) {
-                const int n = min(32, a.group - g0);
-                __syncthreads();
-                if (t < n) {
-                    // head tile h of sequence b has units before·heads + h·chunks + [0, chunks)
-                    const long long u = s.before * heads + (long long)(s.h + (g0 + t) / R) * s.chunks;
-                    sh.w.first[t] = s.owner(u + s.extra);
-                    sh.w.last[t] = s.owner(u + s.chunks - 1);
-                }
-                // four slots a thread at once: their loads do not wait for one another
-                for (int j0 = s.first_slot<kUnit>(s.chunk) + t; j0 - t < end; j0 += 4 * kThreads) {
-                    float sum[4];
+            int held = -1;            // the heads from here have their rows in shared memory
+            // four slots a thread at once: their loads do not wait for one another
+            for (int j0 = s.first_slot<kUnit>(s.chunk) + t; j0 - t < end; j0 += 4 * kThreads) {
+                float sum[4], add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[i] = j0 + i * kThreads < end ? w[j0 + i * kThreads] : 0.f;
-                    if (j0 - t == s.first_slot<kUnit>(s.chunk)) {
+                for (int i = 0; i < 4; ++i) sum[i] = j0 + i * kThreads < end ? w[j0 + i * kThreads] : 0.f;
+                for (int g0 = 0; g0 < a.group; g0 += 32) {
+                    const int n = min(32, a.group - g0);
+                    if (held != g0) {
+                        held = g0;
+                        __syncthreads();
+                        if (t < n) {
+                            // head tile h of sequence b has units before·heads + h·chunks + [0, chunks)
+                            const long long u = s.before * heads + (long long)(s.h + (g0 + t) / R) * s.chunks;
+                            sh.w.first[t] = s.owner(u + s.extra);
+                            sh.w.last[t] = s.owner(u + s.chunks - 1);
+                        }
                         if (!waited) wait_before();
                         waited = true;
                         __syncthreads();
@@ -814,23 +816,22 @@ __global__ void __launch_bounds__(kThreads, 8) attention_join(AttnArgs a, int ro
                         }
                         __syncthreads();
                     }
-                    float add[4] = {0.f, 0.f, 0.f, 0.f};
                     for (int g = 0; g < n; ++g) {
                         const float2 x = sh.w.row[g];
                         const float* sc = a.scores + (row0 + g0 + g) * a.c.slots;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (j0 + i * kThreads < end) 
+                            if (j0 + i * kThreads < end)
                                 add[i] = fmaf(exp2f(fmaf(sc[j0 + i * kThreads], a.scale2, -x.x)), x.y, add[i]);
                     }
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = j0 + i * kThreads;
-                        if (j >= end) continue;
-                        // a row that is not finite gives its slots NaN, but none to those without a page
-                        if (add[i] != add[i] && a.c.offset(a.c.table + (int64_t)s.b * a.c.max_pages, j) < 0) add[i] = 0.f;
-                        if (add[i] != 0.f) w[j] = sum[i] + add[i];
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + i * kThreads;
+                    if (j >= end) continue;
+                    // a row that is not finite gives its slots NaN, but none to those without a page
+                    if (add[i] != add[i] && a.c.offset(a.c.table + (int64_t)s.b * a.c.max_pages, j) < 0) add[i] = 0.f;
+                    if (add[i] != 0.f) w[j] = sum[i] + add[i];
                 }
             }
         }

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from _util import to_dev, to_np, torch_dtype
-from test_gpu_paged import U
+from test_gpu_paged import Cache, U, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +225,38 @@ def test_documented_decode_loop_keeps_its_tokens(budget):
             assert torch.equal(ns["v_cache"][table[b, at // page_size], :, at % page_size], v[b, :, 0])
         assert (ns["weights"][:, :, at] > 0).all()
     assert evictions >= 3
+
+
+# ------------------------------------------- kernel variants that take shapes of their own
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("E", [16, 32, 64, 128])
+@pytest.mark.parametrize("group", [1, 8, 12, 16, 24, 40])
+@pytest.mark.parametrize("PS", [1, 3, 8, 20])
+def test_pages_that_do_not_hold_whole_tiles(dtype, E, group, PS):
+    """Pages that no tile of 16 keys fits: every width and group (one or two head tiles a
+    warp, one or two warps a key group), parts of one tile and sequences split over CTAs."""
+    check_attention(Cache(E + group + PS, dtype, 1, E, PS, [0, 1, 333, 700]), group, weigh=group != 8)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("E,group", [(16, 40), (32, 12), (64, 2), (128, 12), (128, 24)])
+@pytest.mark.parametrize("PS", [7, 8])
+def test_odd_pages_split_over_ctas(dtype, E, group, PS):
+    check_attention(Cache(E + group, dtype, 2, E, PS, [9001, 0, 3000]), 2 * group, weigh=True, scale_q=3.0)
+
+
+@pytest.mark.parametrize("dtype,group", [("f32", 3), ("f32", 12), ("bf16", 3), ("f16", 12), ("bf16", 24), ("f16", 40)])
+@pytest.mark.parametrize("E", [32, 128])
+@pytest.mark.parametrize("PS", [3, 8, 16, 32])
+def test_tables_with_holes(dtype, group, E, PS):
+    """Entries without a page among pages that are there, at the ends and one after
+    another, within a warp's step and over a split."""
+    MP = -(-3000 // PS)
+
+    def holes(table, P):
+        table[0, 1::2] = np.resize([-1, P, 2 ** 31 - 1, -2 ** 31], table[0, 1::2].shape)
+        table[1, 2:5], table[1, -3:], table[1, MP // 2] = -7, P, -1
+        table[2, 0], table[2, 1:4:2] = P + 1, -1
+        table[3, :] = -1
+    check_attention(Cache(E + PS, dtype, 1, E, PS, [MP * PS, 3000 - 1, 77, 500], MP=MP, bad=holes), group, weigh=True)
