@@ -14,8 +14,9 @@
 namespace nnop {
 namespace paged {
 
-// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by a multiplication (round-up method:
-// m = floor(2^32·(2^s − d)/d) + 1 with s = ceil(log2 d)).
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by a multiplication: the round-up method of
+// Granlund and Montgomery, "Division by Invariant Integers using Multiplication" (1994),
+// m = floor(2^32·(2^s − d)/d) + 1 with s = ceil(log2 d).
 struct FastDiv {
     uint32_t d = 1, m = 1;
     int s = 0;
@@ -24,7 +25,9 @@ struct FastDiv {
         while (s < 31 && (1u << s) < div) ++s;
         m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - div)) / div + 1);
     }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return ((uint32_t)(((uint64_t)m * n) >> 32) + n) >> s;
+    }
 };
 
 struct Cache {
@@ -91,7 +94,7 @@ int guarded(const char* who, F&& body) {
 constexpr int kThreads = 128;
 
 // n / d of numbers that mostly fit 32 bits.
-__device__ __forceinline__ long long div_small(long long n, long long d) {
+__host__ __device__ __forceinline__ long long div_small(long long n, long long d) {
     if (((unsigned long long)(n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
     return n / d;
 }
@@ -111,11 +114,11 @@ struct Split {
     int b, h, chunk, chunks, len;
     long long before;      // units / heads in front of sequence b
 
-    __device__ __forceinline__ static long long start(long long units, int c, int G) {
+    __host__ __device__ __forceinline__ static long long start(long long units, int c, int G) {
         return div_small(units * c, G);
     }
     // The CTA that has unit e: the largest c with start(c) <= e.
-    __device__ __forceinline__ int owner(long long e) const {
+    __host__ __device__ __forceinline__ int owner(long long e) const {
         return (int)div_small((e + 1) * G + units - 1, units) - 1;
     }
     template <int kUnit>

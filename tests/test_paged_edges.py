@@ -99,3 +99,50 @@ def test_documented_bindings_have_the_signatures_of_the_library():
         assert [of(t) for t in types] == list(argtypes) and of(result) == res, name
         seen.add(name)
     assert {n for n in SIGNATURES if n.startswith("nnop_paged")} <= seen
+
+
+def test_page_division_and_split_as_compiled(tmp_path):
+    """FastDiv and the split's start() and owner() themselves, compiled for the host:
+    against division, and against a walk over all units."""
+    import ctypes as C
+
+    import numpy as np
+    from nnop import _build
+    src, so = tmp_path / "split.cu", tmp_path / "split.so"
+    src.write_text("""
+        #include "paged.cuh"
+        using namespace nnop::paged;
+        extern "C" void divide(uint32_t d, const uint32_t* n, uint32_t* out, int count) {
+            const FastDiv f(d);
+            for (int i = 0; i < count; ++i) out[i] = f.div(n[i]);
+        }
+        extern "C" long long start(long long units, int c, int G) { return Split::start(units, c, G); }
+        extern "C" int owner(long long units, int G, long long e) {
+            Split s{};
+            s.units = units, s.G = G;
+            return s.owner(e);
+        }
+    """)
+    subprocess.run([_build.nvcc(), *_build.NVCC_FLAGS, "-shared", str(src), "-o", str(so)], check=True, timeout=300)
+    lib = C.CDLL(str(so))
+    lib.divide.argtypes = [C.c_uint32, C.c_void_p, C.c_void_p, C.c_int]
+    lib.start.argtypes, lib.start.restype = [C.c_longlong, C.c_int, C.c_int], C.c_longlong
+    lib.owner.argtypes = [C.c_longlong, C.c_int, C.c_longlong]
+    rng = np.random.default_rng(3)
+    for d in [1, 2, 3, 5, 7, 16, 20, 24, 64, 127, 129, 641, 6700417, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1024,
+              *map(int, rng.integers(1, 2 ** 31 - 1, 100))]:
+        near = [x for k in (0, 1, 2, 2 ** 31 // d - 1, 2 ** 31 // d) for x in (k * d - 1, k * d, k * d + 1)]
+        n = np.array([x for x in [*near, 2 ** 31 - 1, *rng.integers(0, 2 ** 31, 200)] if 0 <= x < 2 ** 31], np.uint32)
+        out = np.zeros_like(n)
+        lib.divide(d, n.ctypes.data, out.ctypes.data, len(n))
+        assert np.array_equal(out, n // np.uint32(d)), d
+    for units, G in [(1, 1), (7, 7), (7, 3), (443, 443), (444, 444), (1000, 444), (12345, 444), (3, 1), (99999, 296)]:
+        starts = [lib.start(units, c, G) for c in range(G + 1)]
+        assert starts[0] == 0 and starts[-1] == units and all(a < b for a, b in zip(starts, starts[1:]))
+        owners = np.searchsorted(starts, np.arange(units), side="right") - 1
+        assert [lib.owner(units, G, e) for e in range(units)] == owners.tolist()
+    for units, G in [(9 * 10 ** 15, 444), (2 ** 40 + 12345, 444)]:          # past 32 bits, at the most the host lets through
+        for c in (0, 1, 100, 443):
+            a, b = lib.start(units, c, G), lib.start(units, c + 1, G)
+            assert a == units * c // G and b == units * (c + 1) // G
+            assert lib.owner(units, G, a) == c == lib.owner(units, G, b - 1)
