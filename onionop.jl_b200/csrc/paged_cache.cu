@@ -386,48 +386,28 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select(EvictArgs a, int 
 }
 
 constexpr int kMoveBlock = 256;
-constexpr int kMoveRows = 1;
 
 // Moves the kept rows of one KV head (blockIdx.y) of one sequence (blockIdx.z): a thread
-// has one 16-byte vector of K and of V in each of kMoveRows rows, all loaded before any
-// is stored.
+// has one 16-byte vector of K and of V of one row, both loaded before either is stored.
 template <typename T, int E>
 __global__ void __launch_bounds__(kMoveBlock) evict_move(EvictArgs a) {
     constexpr int VEC = 16 / sizeof(T), NV = E / VEC, PER = kMoveBlock / NV;
     wait_before();
     const int64_t b = blockIdx.z;
-    const int e = threadIdx.x % NV * VEC;
-    const int at0 = blockIdx.x * (PER * kMoveRows) + threadIdx.x / NV;
+    const int64_t row = b * a.KH + blockIdx.y;
+    const int e = threadIdx.x % NV * VEC, at = blockIdx.x * PER + threadIdx.x / NV;
+    const int slot = at < a.budget ? a.kept[row * a.budget + at] : -1;
+    if (slot < 0) return;
+    if (e == 0) a.new_weights[row * a.new_slots + at] = a.weights[row * a.c.slots + slot];
     const int64_t ho = blockIdx.y * a.c.head_stride + e;
-    const int* kept = a.kept + (b * a.KH + blockIdx.y) * a.budget;
-    const T* K = static_cast<const T*>(a.k_cache);
-    const T* V = static_cast<const T*>(a.v_cache);
-    int64_t to[kMoveRows];
-    Vec<T, VEC> x[kMoveRows], y[kMoveRows];
-#pragma unroll
-    for (int j = 0; j < kMoveRows; ++j) {
-        const int at = at0 + j * PER;
-        const int slot = at < a.budget ? kept[at] : -1;
-        to[j] = -1;
-        if (slot >= 0) {
-            if (e == 0) {
-                const int64_t row = b * a.KH + blockIdx.y;
-                a.new_weights[row * a.new_slots + at] = a.weights[row * a.c.slots + slot];
-            }
-            const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot);
-            if (from >= 0) {
-                to[j] = a.c.offset(a.new_table + b * a.new_max_pages, at);
-                x[j] = ldg_stream<T, VEC>(K + from + ho);
-                y[j] = ldg_stream<T, VEC>(V + from + ho);
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < kMoveRows; ++j)
-        if (to[j] >= 0) {
-            st_stream<T, VEC>(static_cast<T*>(a.k_cache) + to[j] + ho, x[j]);
-            st_stream<T, VEC>(static_cast<T*>(a.v_cache) + to[j] + ho, y[j]);
-        }
+    const int64_t from = a.c.offset(a.c.table + b * a.c.max_pages, slot);
+    if (from < 0) return;
+    const int64_t to = a.c.offset(a.new_table + b * a.new_max_pages, at);
+    const Vec<T, VEC> x = ldg_stream<T, VEC>(static_cast<const T*>(a.k_cache) + from + ho);
+    const Vec<T, VEC> y = ldg_stream<T, VEC>(static_cast<const T*>(a.v_cache) + from + ho);
+    if (to < 0) return;
+    st_stream<T, VEC>(static_cast<T*>(a.k_cache) + to + ho, x);
+    st_stream<T, VEC>(static_cast<T*>(a.v_cache) + to + ho, y);
 }
 
 int launch_select(const EvictArgs& a, cudaStream_t s) {
@@ -468,7 +448,7 @@ int launch_select(const EvictArgs& a, cudaStream_t s) {
 
 template <typename T, int E>
 int launch_evict(const EvictArgs& a, cudaStream_t s) {
-    constexpr int kRows = kMoveBlock / (E / (16 / (int)sizeof(T))) * kMoveRows;      // per block
+    constexpr int kRows = kMoveBlock / (E / (16 / (int)sizeof(T)));      // per block
     if (const int rc = launch_select(a, s)) return rc;
     if (a.budget == 0) return NNOP_OK;
     const unsigned grid = (unsigned)((a.budget + kRows - 1) / kRows);
