@@ -484,6 +484,9 @@ size_t nnop_paged_attention_fwd_workspace_size(int64_t E, int64_t QH, int64_t KH
  *   q, o [B][QH][E] (QL = 1: the flash-attention layout [B][QH][1][E]);
  *   lse [B][QH] f32.  A sequence without a slot (or whose scores are all -Inf)
  *   gets o = 0, lse = -Inf.
+ *   Elements of k and v that are not finite count in attended slots as in the
+ *   formula (f16: a weight under 2^-38 of the row's largest counts as 0), and
+ *   nowhere else.
  *   weights [B][KH][max_pages*page_size] f32 or NULL: for every attended slot j
  *   weights[b][h][j] += sum over the query heads of kv head h of their softmax
  *   weight on j; other elements are left as they are.

@@ -283,15 +283,14 @@ attention_simt(AttnArgs a) {
 // row (4 lanes read 64 bytes of each of 8 rows), and Q is laid out to match.  The
 // rows of Oᵀ may be any E order too: a lane loads 16 bytes of 4 V rows (8 lanes read
 // 128 bytes of a row) and pairs two keys' halves by byte permutes.  Sᵀ's
-// accumulators become Pᵀ's B fragments by movmatrix.  P keeps fp32's bits: it goes in
-// as the sum of three bf16 terms (24 bits) or two f16 terms (22 bits, less than ex2's
-// own error away).  Rounded once to 16 bits it would cost as much accuracy as rounding
-// the result does.  Of 65536 bf16 results (16 sequences up to 8192) two terms (16 bits)
-// rounded 78 to another side than exact values do, three 47, products in fp32 34; the third
-// term takes 64 such sequences from 168 to 171 us (the launch alone), groups of 16 heads
-// from 111 to 119.
-// f16: P is scaled by 2^14, which the running sum shares, so that weights down to
-// 2^-38 of the largest count.
+// accumulators become Pᵀ's B fragments by movmatrix.  P keeps fp32's bits, to ex2's own
+// error of 2^-22: it goes in as the sum of three bf16 terms or two f16 terms (pack2).
+// Rounded once to 16 bits it would cost as much accuracy as rounding the result does; of
+// 65536 bf16 results (16 sequences up to 8192) two terms rounded 78 to another side than
+// exact values do, three 51, products in fp32 34.  The third term takes 64 sequences up to
+// 8192 with 16 heads a group from 111 to 117 us; 4 heads stay at 169 (the launch alone).
+// f16: P is scaled by 2^14, which the running sum shares, so that weights down to 2^-38 of
+// the largest count.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -325,19 +324,35 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// Two values rounded to T, and what the rounding left of them (rest_lo, rest_hi may be lo, hi).
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi, float& rest_lo, float& rest_hi) {
+// Two values as a pair of T, rounded to nearest or (kRest) towards zero with what that
+// left of them in their place.  The rest of a value above 0 is above 0 too, so that an
+// infinite element of V times each of a probability's terms has one sign: bf16 makes the
+// rest larger by 2^-23 of the probability for that, f16 at least its smallest number, 2^-24
+// (2^-38 of the largest probability).
+template <typename T, bool kRest, int kTerm>
+__device__ __forceinline__ uint32_t pack2(float& lo, float& hi) {
+    uint32_t r;
     if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        rest_lo = lo - __low2float(h);
-        rest_hi = hi - __high2float(h);
-        return *reinterpret_cast<const uint32_t*>(&h);
+        if constexpr (!kRest) {
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+            return r;
+        }
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        const __half2 h = *reinterpret_cast<const __half2*>(&r);
+        lo = fmaxf(lo - __low2float(h), fminf(__low2float(h), 0x1p-24f));
+        hi = fmaxf(hi - __high2float(h), fminf(__high2float(h), 0x1p-24f));
     } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        rest_lo = lo - __low2float(h);
-        rest_hi = hi - __high2float(h);
-        return *reinterpret_cast<const uint32_t*>(&h);
+        if constexpr (!kRest) {
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+            return r;
+        }
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        // the first rest is up to 2^-7 of the probability
+        constexpr float kMore = kTerm == 0 ? 1.f + 0x1p-23f : 1.f + 0x1p-16f;
+        lo = fmaf(lo, kMore, -__uint_as_float(r << 16));
+        hi = fmaf(hi, kMore, -__uint_as_float(r & 0xffff0000u));
     }
+    return r;
 }
 
 template <int E> struct MmaShape {
@@ -607,8 +622,9 @@ attention_mma(AttnArgs a) {
                         float p1 = fast_exp2(fmaf(d[n][t][i * 2 + 1], a.scale2, -base[n][1]));
                         l[n][0] += p0;
                         l[n][1] += p1;
-#pragma unroll
-                        for (int k = 0; k < kTerms; ++k) b[n][t][k][i] = transpose8x8(pack2<T>(p0, p1, p0, p1));
+                        b[n][t][0][i] = transpose8x8(pack2<T, true, 0>(p0, p1));
+                        if constexpr (kTerms == 3) b[n][t][1][i] = transpose8x8(pack2<T, true, 1>(p0, p1));
+                        b[n][t][kTerms - 1][i] = transpose8x8(pack2<T, false, kTerms - 1>(p0, p1));
                     }
             }
 #pragma unroll

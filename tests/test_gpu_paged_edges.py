@@ -20,8 +20,9 @@ def test_probabilities_enter_the_sum_with_32_bits(dtype):
     the probabilities that the rounding of o hides elsewhere.
 
     Scores are exact (one product of two 16-bit numbers; the scale is 1/4): 0 and -x, so
-    the weights are 1 and p = exp(-x).  p is off by ex2's 2^-22, by 2^-22 for what its
-    split into terms may drop, and by 4u·x for the rounding of its argument; v1 + p·v2 by
+    the weights are 1 and p = exp(-x).  p is off by ex2's 2^-22, by 2^-21 for what its
+    split into terms may drop (f16: 2^-10 of it is left by the first, rounded towards zero,
+    and 2^-11 of that by the second; bf16: 2^-7, 2^-7 and 2^-8), and by 4u·x for the rounding of its argument; v1 + p·v2 by
     two half steps of its larger addend, twice (later terms are 2^-8 of it: 1/16 more);
     the division and the rounding of o by their share of o, half a step of f16's smallest
     (2^-25) where o is that small."""
@@ -50,7 +51,7 @@ def test_probabilities_enter_the_sum_with_32_bits(dtype):
                              torch.full((B,), 2, device="cuda", dtype=torch.int32))
     want = (v1 + p * v2) / (1 + p)
     a2 = p * np.abs(v2)
-    tol = (a2 * (2.0 ** -21 + 4 * U * x[:, None]) + 4 * U * np.maximum(np.abs(v1), a2) * (1 + 2.0 ** -4)) / (1 + p)
+    tol = (a2 * (2.0 ** -22 + 2.0 ** -21 + 4 * U * x[:, None]) + 4 * U * np.maximum(np.abs(v1), a2) * (1 + 2.0 ** -4)) / (1 + p)
     tol += (HALF[dtype] + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "f16" else 0)
     over = np.abs(to_np(o)[:, 0, 0] - want) / tol
     assert over.max() <= 1, f"{over.max():.3g} times its tolerance"
@@ -260,3 +261,31 @@ def test_tables_with_holes(dtype, group, E, PS):
         table[2, 0], table[2, 1:4:2] = P + 1, -1
         table[3, :] = -1
     check_attention(Cache(E + PS, dtype, 1, E, PS, [MP * PS, 3000 - 1, 77, 500], MP=MP, bad=holes), group, weigh=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("E,group,PS", [(16, 1, 16), (32, 12, 3), (64, 40, 16), (128, 4, 16), (128, 4, 20)])
+@pytest.mark.parametrize("n", [1, 30, 20000])
+def test_values_that_are_not_finite(dtype, E, group, PS, n):
+    """An infinite element of v in an attended slot makes its column of o that infinity,
+    whatever the bits of the slot's weight; NaN, or both infinities, make it NaN; the other
+    columns keep their values."""
+    import torch
+
+    import nnop
+    c = Cache(60, dtype, 1, E, PS, [n, n])
+    q = to_dev(c.rng.standard_normal((2, group, 1, E)), dtype)
+    put = lambda b, slot, e, x: c.v[int(c.table[b, slot // PS]), 0, slot % PS].__setitem__(e, x)  # noqa: E731
+    before, _ = nnop._paged_attention(q, *c.args)
+    put(0, 0, 0, math.inf), put(0, n - 1, 1, -math.inf), put(0, n // 2, 2, math.nan)
+    for slot in range(min(n, 40)):
+        put(0, slot, 3, math.inf)
+    put(0, n // 2, 4, math.inf), put(0, n - 1, 4, -math.inf)
+    if n > 1:
+        put(0, 0, 4, -math.inf)
+    o, _ = nnop._paged_attention(q, *c.args)
+    assert torch.equal(o[1], before[1]) and torch.equal(o[0, :, :, 5:], before[0, :, :, 5:])
+    o = to_np(o)[0, :, 0]
+    assert (o[:, 0] == math.inf).all() and (o[:, 1] == -math.inf).all() and np.isnan(o[:, 2]).all()
+    assert (o[:, 3] == math.inf).all()
+    assert np.isnan(o[:, 4]).all() if n > 1 else (o[:, 4] == -math.inf).all()
