@@ -4,17 +4,23 @@
 // group reading the same rows.  Optionally weights[b][kv head][j] += Σ over the
 // group's heads of softmax(s)_j, which is what nnop_paged_evict goes by.
 //
-// Bound: HBM.  Each cached row is read once for all query heads of its group,
-// 2·Σ lengths·KH·E·size bytes, against 4·Σ lengths·QH·E flops.
+// Bound: HBM.  Each cached row is read once for all query heads of its group, 2·Σ
+// lengths·KH·E·size bytes, against 4·Σ lengths·QH·E flops, where the group fits a head
+// tile of R heads: 8, 16 or 32 in 16 bits, 1 to 8 in fp32 (rows_per_tile).  A larger
+// group's rows are read once per tile, ceil(group / R) times; with tiles of 32 the two
+// warps of a key group each load them, the second time mostly from L2.
+//
+// Times in this file are the launches' alone (CUDA events, calls queued behind one
+// another); a call through the Python mirror takes about 3 us more where it is large.
 //
 // One launch splits the batch evenly over its CTAs whatever the lengths are
 // (paged.cuh).  A CTA runs a softmax over its part of a sequence with a running
 // maximum and sum, every warp on keys of its own, and joins its warps through
 // shared memory.  A (sequence, head tile) that lies in one CTA is written at once;
 // the others leave (maximum, sum, accumulator) in the workspace and a second launch
-// joins them.  The weights need the final lse, so the scores are kept (fp32,
-// workspace) and the second launch turns them into weights: 8 bytes per (query head,
-// slot) instead of reading K again (E·size).
+// joins them.  The weights need the final maximum and sum, so the scores are kept
+// (fp32, workspace) and the second launch turns them into weights: 8 bytes per (query
+// head, slot) instead of reading K again (E·size).
 #include "paged.cuh"
 
 #include <cmath>
@@ -83,8 +89,8 @@ constexpr int kSimtExtra = 8;      // units that a segment's begin and end cost 
 // fp32 (no tensor cores: their formats would cost its accuracy): a quad of lanes per key
 // for the scores, E/32 columns per lane for the products with V, R query heads per pass
 // over the keys.  A step's rows are all in flight before any is used, K of the next step
-// while this one's softmax runs, V while the next scores do: loads under a branch, one
-// at a time, took 259 us where this takes 104 (16 sequences up to 8192, 32/8 heads of 128).
+// while this one's softmax runs, V while the next scores do: 107 us (16 sequences up to
+// 8192, 32/8 heads of 128, 538 MB); loads under a branch, one at a time, took 259.
 template <int E, int R>
 __global__ void __launch_bounds__(kThreads, 3)
 attention_simt(AttnArgs a) {
@@ -270,9 +276,9 @@ attention_simt(AttnArgs a) {
 
 // ---------------------------------------------------------------------------
 // Tensor-core kernel for the 16-bit types (mma.sync m16n8k16).  The op is bound by
-// HBM: at 8 query heads a key row it needs 1/6 of mma.sync's rate, so what matters
-// is that the loads never stop, and the operands go from global memory straight
-// into the fragments -- no shared memory, no barrier, every warp on its own keys:
+// HBM (with up to 8 query heads a key row the tensor pipe is busy 15% of the time),
+// so what matters is that the loads never stop, and the operands go from global
+// memory straight into the fragments -- no shared memory, no barrier, every warp on its own keys:
 //
 //   Sᵀ (16 keys × 8 heads) = K (A: 16 × E) · Qᵀ (B: E × 8)
 //   Oᵀ (E × 8 heads)      += Vᵀ (A: E × 16 keys) · Pᵀ (B: 16 keys × 8)
@@ -362,15 +368,17 @@ template <int E> struct MmaShape {
 };
 
 // CTAs per SM.  What has to be in flight to keep HBM busy lies in registers, 8 KB a
-// warp, beside 32·NT for Oᵀ and 16·NT for Q: three CTAs of 168 registers a thread
-// (168 us for 64 sequences up to 8192) before two of 255 (174 us) or four that spill
-// (254 us); with two head tiles a warp, two.  A ring in shared memory filled by cp.async,
-// with up to 192 KB in flight, was slower: 173 us, and 107 instead of 90 for heads of 64.
+// warp, beside 32·NT for Oᵀ and 16·NT for Q: three CTAs of 168 registers a thread, which
+// spill 24 bytes at most (170 us for 64 sequences up to 8192, heads of 64 91 us, of 32 57),
+// before two of 255 (177, 99, 66) or four of 128, which spill all they hold (216, 94, 58);
+// with two head tiles a warp, two.  A ring in shared memory filled by cp.async, with up to
+// 192 KB in flight, was slower when it was tried: 173 us where this took 167, and 107
+// instead of 90 for heads of 64.
 constexpr int mma_ctas(int NT) { return NT == 1 ? 3 : 2; }
 // What a segment's begin and end count for, in units (8 KB; a CTA among two has a larger
-// share of HBM than one among three).  64 sequences up to 8192: 2 units 172 us, 4 units
-// 168, 8 units 167; 32 of them with two head tiles: 8 units 132 us, 12 units 123, 16 units
-// 110, 24 units 109.
+// share of HBM than one among three).  64 sequences up to 8192: 2 units 179 us, 4 units
+// 172, 8 units 170; 32 of them with two head tiles: 8 units 142 us, 12 units 130, 16 units
+// 117, 24 units 119.
 constexpr int mma_extra(int NT) { return NT == 1 ? 8 : 16; }
 
 // NT: head tiles (of 8) per warp, which share the fragments of K and V.  WT: warps
@@ -409,9 +417,9 @@ attention_mma(AttnArgs a) {
 
     // Where a step's rows are.  kWholeTiles (pages of a multiple of 16 slots): a tile of 16
     // keys lies in one page, one lookup for all lanes, its table entry fetched a step ahead
-    // (168 us for 64 sequences up to 8192; 175 when it is fetched with the rows).  Else one
-    // lookup for each row a lane reads (pages of 20: 169 us, but heads of 64 in pages of 16
-    // would take 107 us that way instead of 90, heads of 32 93 instead of 54).
+    // (fetched with the rows it took 175 us instead of 168 for 64 sequences up to 8192).  Else
+    // one lookup for each row a lane reads (pages of 20: 171 us as against 170, but heads of
+    // 64 in pages of 16 would take 111 us that way instead of 91, heads of 32 96 instead of 57).
     uint32_t page[S::kTiles];      // table entries of the next step's tiles
     int row[S::kTiles];
     int64_t tiles[S::kTiles] = {}; // bytes into the pool; negative: no page
@@ -535,7 +543,7 @@ attention_mma(AttnArgs a) {
         }
         for (; key0 < end; key0 += kStep) {
             // Pages of other sizes: each chunk's registers are loaded again as soon as its
-            // products are through (pages of 20: 169 us instead of 179).
+            // products are through (pages of 20: 169 us instead of 179 when it was tried).
             const bool more = key0 + kStep < end;
             uint32_t next = ~0u;
             if (more) found(key0 + kStep);

@@ -74,8 +74,9 @@ constexpr int kAppendHeads = 4;      // heads per thread
 // E/2 further on (the pair that RoPE rotates) for kAppendHeads heads of q, of k or of v
 // (blockIdx.y): the angles, the page and the index arithmetic are fetched once for all
 // of them, and all rows are loaded before any is used.  Four prompts of 8192 tokens (32 +
-// 8 heads of 128, bf16, 772 MB): 117 us, 6.59 TB/s, with streaming stores; 175 us with
-// plain ones, 126 with two heads per thread, 117 with eight.
+// 8 heads of 128, bf16, 772 MB), the launch alone: 117 us, 6.59 TB/s, with streaming stores
+// (a call through the Python mirror: 121 us, 6.4 TB/s); 175 us with plain ones, 126 with
+// two heads per thread, 117 with eight.
 template <typename T, int E>
 __global__ void __launch_bounds__(kAppendBlock) append_kernel(AppendArgs a) {
     constexpr int VEC = 16 / sizeof(T), HALF = E / 2, NH = HALF / VEC;
