@@ -876,7 +876,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, weights=None):
     not attended to; a sequence without a slot gets zeros).  ``weights``
     (B, KH, MP·PS) float32, contiguous: each attended slot's softmax weight,
     summed over the query heads of its kv head, is added to it in place --
-    what ``paged_evict`` goes by."""
+    what ``paged_evict`` goes by; the call then takes a workspace of 4 bytes per
+    query head and slot of the table, whatever the lengths."""
     return _paged_attention(q, k_cache, v_cache, block_table, lengths, weights=weights)[0]
 
 
