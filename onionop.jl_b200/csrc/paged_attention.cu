@@ -10,8 +10,7 @@
 // group's rows are read once per tile, ceil(group / R) times; with tiles of 32 the two
 // warps of a key group each load them, the second time mostly from L2.
 //
-// Times in this file are the launches' alone (CUDA events, calls queued behind one
-// another); a call through the Python mirror takes about 3 us more where it is large.
+// Times in this file are of CUDA events around calls queued behind one another.
 //
 // One launch splits the batch evenly over its CTAs whatever the lengths are
 // (paged.cuh).  A CTA runs a softmax over its part of a sequence with a running
